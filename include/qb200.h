@@ -47,8 +47,9 @@ typedef enum qb200_status {
 } qb200_status;
 
 /* One floating dtype per plan; mixed programs are rejected
- * (cuda.rs:998-1030, cuda_real.rs:151-210). */
-typedef enum qb200_dtype { QB200_F32 = 0, QB200_F64 = 1 } qb200_dtype;
+ * (cuda.rs:998-1030, cuda_real.rs:151-210).  The 16-bit dtypes are for the stand-alone layer
+ * norm and dropout alone: every other entry point refuses them. */
+typedef enum qb200_dtype { QB200_F32 = 0, QB200_F64 = 1, QB200_F16 = 2, QB200_BF16 = 3 } qb200_dtype;
 
 typedef enum qb200_param_kind { QB200_WEIGHT = 0, QB200_BIAS = 1 } qb200_param_kind;
 
@@ -414,6 +415,97 @@ qb200_status qb200_matmul_3xtf32(const void* d_a, const void* d_w, const void* d
  * ------------------------------------------------------------------------ */
 qb200_status qb200_weight_gradient_static(int32_t dtype, const void* d_acts, const void* d_cots, int64_t rows,
                                           int32_t d_in, int32_t d_out, void* d_grad, void* cuda_stream);
+
+/* ------------------------------------------------------------------------
+ * Stand-alone dropout, layer norm and their residual form, forward and
+ * backward, over caller-owned device arrays.  No counterpart in the reference
+ * (its networks are plain multi-layer perceptrons); the dropout mask comes from
+ * its generator.
+ *
+ * Arrays of rows hold `rows` x `cols` elements of `dtype` (any of the four), a
+ * row's elements next to each other, row r at data + r * stride elements.
+ * Strides of arrays that are read are >= 0 (0 repeats one row), of arrays that
+ * are written >= cols; with one row the stride is not looked at.  Pointers need
+ * the alignment of one element; rows that start on 16-byte boundaries in every
+ * array of a call take the wide path, others are read and written one element
+ * at a time.  What lies between cols and the stride is neither read nor
+ * written.  Zero rows are valid (the sums over rows are then zero).  Parameters
+ * (weight, bias and their gradients) are of `param_dtype`: the rows' dtype, or
+ * QB200_F32 beside 16-bit rows; either may be NULL and then stands for 1 or 0.
+ * Statistics (mean, rstd) and all sums are float32, float64 for float64 rows;
+ * results are rounded to their type once.  Sums run in a fixed order: the same
+ * call gives the same bits.
+ *
+ * The calls enqueue kernels on the given stream and return; they allocate
+ * nothing, keep nothing and can be captured into a graph.  They run on the
+ * device that holds the (first) row array, whichever is current; every array
+ * of a call and the stream belong to that device.  Results may take the place
+ * of a row array that is read, with the same stride (y for x or residual, h
+ * for residual or x; dx or dresidual for dy, dh or h); two results may not
+ * share memory, nor may arrays overlap in another way.
+ *
+ * Rows of layer norm hold at most 65,536 elements (32,768 in float64;
+ * QB200_TOO_LARGE above), dropout's any number.
+ * ------------------------------------------------------------------------ */
+
+/* y = kept ? x / (1 - rate) : 0, rate in [0, 1).  Dropped elements are 0 whatever x holds.
+ * Element (r, c) has index e = counter + *d_counter + r * cols + c and is kept iff the low
+ * (e even) or high (e odd) 32 bits of word e / 2 of the key's SplitMix64 stream (the stream of
+ * quabla_b200.random) are >= floor(rate * 2^32); indices stay below 2^64 (refused where
+ * counter alone passes it).  The mask is not stored: the backward pass is
+ * the same call on the gradient.  d_counter (NULL: 0) is read when the kernel runs, so a
+ * captured step draws a new mask each time it is replayed after the word was advanced.
+ * quabla_b200.random.dropout_mask(key, shape, rate, counter) is the mask on the host. */
+qb200_status qb200_dropout(int32_t dtype, const void* d_x, int64_t x_stride, int64_t rows, int64_t cols, double rate,
+                           uint64_t key, uint64_t counter, const uint64_t* d_counter, void* d_y, int64_t y_stride,
+                           void* cuda_stream);
+
+/* y = (x - mean) * rstd * weight + bias, mean and variance over each row's columns,
+ * rstd = 1 / sqrt(variance + epsilon).  mean and rstd ([rows], either may be NULL) are what the
+ * backward pass needs. */
+qb200_status qb200_layer_norm(int32_t dtype, int32_t param_dtype, const void* d_x, int64_t x_stride, int64_t rows,
+                              int32_t cols, const void* d_weight, const void* d_bias, double epsilon, void* d_y,
+                              int64_t y_stride, void* d_mean, void* d_rstd, void* cuda_stream);
+
+/* Bytes of workspace of a backward pass over `rows` x `cols` (at most 19 MiB): partial sums of
+ * the parameters' gradients, one row for each group of thread blocks. */
+qb200_status qb200_layer_norm_workspace(int32_t dtype, int64_t rows, int32_t cols, size_t* nbytes);
+
+/* With xh = (x - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - mean(g) - xh * mean(g * xh)),  dweight = sum over rows of dy * xh,
+ *   dbias = sum over rows of dy.
+ * dweight and dbias ([cols], written, not added to) may each be NULL; with both NULL there need
+ * be no workspace.  The workspace (16-byte aligned, its contents neither read nor kept) belongs
+ * to the call until its kernels have run: calls that may run at the same time, among them
+ * replays of graphs, need one each. */
+qb200_status qb200_layer_norm_backward(int32_t dtype, int32_t param_dtype, const void* d_dy, int64_t dy_stride,
+                                       const void* d_x, int64_t x_stride, int64_t rows, int32_t cols,
+                                       const void* d_weight, const void* d_mean, const void* d_rstd, void* d_dx,
+                                       int64_t dx_stride, void* d_dweight, void* d_dbias, void* d_workspace,
+                                       size_t workspace_bytes, void* cuda_stream);
+
+/* h = residual + dropout(x), y = layer_norm(h), in one pass.  residual may be NULL (h =
+ * dropout(x)), and so may h where no backward pass follows.  Statistics and y are of h before it
+ * is rounded to dtype. */
+qb200_status qb200_dropout_layer_norm(int32_t dtype, int32_t param_dtype, const void* d_x, int64_t x_stride,
+                                      const void* d_residual, int64_t residual_stride, int64_t rows, int32_t cols,
+                                      double rate, uint64_t key, uint64_t counter, const uint64_t* d_counter,
+                                      const void* d_weight, const void* d_bias, double epsilon, void* d_h,
+                                      int64_t h_stride, void* d_y, int64_t y_stride, void* d_mean, void* d_rstd,
+                                      void* cuda_stream);
+
+/* dy is the gradient of y, dh (may be NULL) the one that reaches h along its other uses:
+ *   dresidual = layer_norm_backward(dy) + dh (may be NULL),  dx = kept ? dresidual / (1 - rate) : 0
+ * with the mask of the forward call's rate, key and counters.  The rest as in
+ * qb200_layer_norm_backward. */
+qb200_status qb200_dropout_layer_norm_backward(int32_t dtype, int32_t param_dtype, const void* d_dy, int64_t dy_stride,
+                                               const void* d_dh, int64_t dh_stride, const void* d_h, int64_t h_stride,
+                                               int64_t rows, int32_t cols, const void* d_weight, const void* d_mean,
+                                               const void* d_rstd, double rate, uint64_t key, uint64_t counter,
+                                               const uint64_t* d_counter, void* d_dx, int64_t dx_stride,
+                                               void* d_dresidual, int64_t dresidual_stride, void* d_dweight,
+                                               void* d_dbias, void* d_workspace, size_t workspace_bytes,
+                                               void* cuda_stream);
 
 #ifdef __cplusplus
 }

@@ -13,7 +13,7 @@ import os
 from . import _build
 
 OK, INVALID, UNSUPPORTED, CUDA_ERROR, NCCL_ERROR, NOT_BOUND, TOO_LARGE = range(7)
-F32, F64 = 0, 1
+F32, F64, F16, BF16 = 0, 1, 2, 3
 WEIGHT, BIAS = 0, 1
 ACT_TANH, ACT_SIN, ACT_SIGMOID, ACT_SOFTPLUS, ACT_SILU, ACT_GELU = range(6)
 ACTIVATIONS = {"tanh": ACT_TANH, "sin": ACT_SIN, "sigmoid": ACT_SIGMOID, "softplus": ACT_SOFTPLUS, "silu": ACT_SILU,
@@ -64,6 +64,8 @@ class BackendError(RuntimeError):
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
+_U64 = C.c_uint64
+_F64 = C.c_double
 SIGNATURES = {
     "qb200_last_error": (C.c_char_p, []),
     "qb200_version": (C.c_char_p, []),
@@ -117,6 +119,15 @@ SIGNATURES = {
     "qb200_optimizer_apply": (_I32, [_I32, _P, _P, _P, _P, _I64, C.POINTER(OptConfig), _I64, _P]),
     "qb200_weight_gradient": (_I32, [_I32, _P, _P, _I64, _I32, _I32, _P, _P]),
     "qb200_weight_gradient_static": (_I32, [_I32, _P, _P, _I64, _I32, _I32, _P, _P]),
+    "qb200_dropout": (_I32, [_I32, _P, _I64, _I64, _I64, _F64, _U64, _U64, _P, _P, _I64, _P]),
+    "qb200_layer_norm": (_I32, [_I32, _I32, _P, _I64, _I64, _I32, _P, _P, _F64, _P, _I64, _P, _P, _P]),
+    "qb200_layer_norm_workspace": (_I32, [_I32, _I64, _I32, C.POINTER(C.c_size_t)]),
+    "qb200_layer_norm_backward": (_I32, [_I32, _I32, _P, _I64, _P, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P, _P, _P,
+                                         C.c_size_t, _P]),
+    "qb200_dropout_layer_norm": (_I32, [_I32, _I32, _P, _I64, _P, _I64, _I64, _I32, _F64, _U64, _U64, _P, _P, _P, _F64, _P,
+                                        _I64, _P, _I64, _P, _P, _P]),
+    "qb200_dropout_layer_norm_backward": (_I32, [_I32, _I32, _P, _I64, _P, _I64, _P, _I64, _I64, _I32, _P, _P, _P, _F64,
+                                                 _U64, _U64, _P, _P, _I64, _P, _I64, _P, _P, _P, C.c_size_t, _P]),
     "qb200_matmul_3xtf32": (_I32, [_P, _P, _P, _P, _I64, _I32, _I32, _I64, _P]),
 }
 

@@ -1,0 +1,91 @@
+// Arguments and launch shapes of the stand-alone layer norm, dropout and residual-form kernels, shared by the entry
+// points (norm.cu) and the kernels' translation units (norm_f32.cu, norm_f64.cu, norm_f16.cu, norm_bf16.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "draws.cuh"
+
+namespace qb {
+
+struct RowArray {
+    void* data = nullptr;
+    long long stride = 0;  // elements between rows
+};
+
+struct NormForwardArgs {
+    RowArray x, residual, h, y;  // residual and h may be absent
+    const void* weight = nullptr;
+    const void* bias = nullptr;
+    void* mean = nullptr;
+    void* rstd = nullptr;
+    double epsilon = 0.0;
+    Draw draw;
+    long long rows = 0;
+    int cols = 0;
+    bool params_f32 = false;  // weight and bias are float32 beside 16-bit rows
+};
+
+struct NormBackwardArgs {
+    RowArray dy, dh, h, dx, dresidual;  // dh and dresidual may be absent
+    const void* weight = nullptr;
+    const void* mean = nullptr;
+    const void* rstd = nullptr;
+    void* dweight = nullptr;
+    void* dbias = nullptr;
+    void* partial = nullptr;  // [partials][2][cols] in the accumulation type
+    Draw draw;
+    long long rows = 0;
+    int cols = 0;
+    bool params_f32 = false;
+};
+
+struct DropoutArgs {
+    RowArray x, y;
+    Draw draw;
+    long long rows = 0;
+    long long cols = 0;
+};
+
+// Elements of a row that one thread keeps in registers, and threads of a CTA at most.
+__host__ __device__ constexpr int norm_elements(size_t element_bytes) { return element_bytes == 8 ? 8 : 16; }
+constexpr int NORM_MAX_THREADS = 512;
+constexpr int NORM_MAX_CLUSTER = 8;
+constexpr int NORM_SMS = 148;
+
+// How the rows of an array are laid over threads: `threads_per_row` threads of each of `cluster` CTAs hold a row
+// (columns [rank * slice, (rank + 1) * slice) in CTA `rank`), `groups` rows at once in a CTA.
+struct RowShape {
+    int threads_per_row, groups, cluster, slice;
+};
+
+inline RowShape row_shape(int cols, int elements) {
+    RowShape s{};
+    const int capacity = NORM_MAX_THREADS * elements;
+    s.cluster = 1;
+    while (s.cluster * capacity < cols) s.cluster *= 2;
+    s.slice = ((cols + s.cluster - 1) / s.cluster + elements - 1) / elements * elements;
+    const int needed = s.slice / elements;
+    if (needed <= 32) {
+        s.threads_per_row = 1;
+        while (s.threads_per_row < needed) s.threads_per_row *= 2;
+    } else {
+        s.threads_per_row = (needed + 31) / 32 * 32;
+    }
+    s.groups = s.threads_per_row >= 256 ? 1 : 256 / s.threads_per_row;
+    return s;
+}
+
+// Rows of partial weight gradients that a backward pass leaves (one per cluster of CTAs).
+inline int norm_partials(long long rows, const RowShape& s) {
+    const long long batches = (rows + s.groups - 1) / s.groups;
+    const int resident = NORM_SMS * (s.threads_per_row * s.groups <= 256 ? 2 : 1) / s.cluster;
+    return (int)(batches < resident ? batches : resident);
+}
+
+template <typename T> cudaError_t norm_forward_launch(const NormForwardArgs& a, cudaStream_t stream);
+template <typename T> cudaError_t norm_backward_launch(const NormBackwardArgs& a, cudaStream_t stream);
+template <typename T> cudaError_t dropout_launch(const DropoutArgs& a, cudaStream_t stream);
+
+}  // namespace qb

@@ -10,7 +10,9 @@ lets NumPy generate whole arrays at once.
            u = ((bits >> 11) + 0.5) / 2^53 (tensor.rs:336-345, 1436-1454);
   glorot   normal * sqrt(2 / (fan_in + fan_out)) (python/quabla/random.py:197-204);
   split    the next `num` outputs of the stream (tensor.rs:1426-1433);
-  fold_in  mix(key ^ mix-stream(data)) (tensor.rs:1539-1543).
+  fold_in  mix(key ^ mix-stream(data)) (tensor.rs:1539-1543);
+  dropout_mask  32 bits of the stream per element, the mask that the device's
+           dropout entry points draw (qb200_dropout; not in the reference).
 """
 
 from __future__ import annotations
@@ -54,10 +56,10 @@ def _mix_scalar(z: int) -> int:
     return z ^ (z >> 31)
 
 
-def _stream(key: int, count: int) -> np.ndarray:
-    """The first `count` outputs of the SplitMix64 stream seeded by `key`."""
+def _stream(key: int, count: int, first: int = 0) -> np.ndarray:
+    """`count` outputs of the SplitMix64 stream seeded by `key`, from output `first` on."""
     with np.errstate(over="ignore"):
-        z = np.uint64(key) + np.arange(1, count + 1, dtype=np.uint64) * np.uint64(_GAMMA)
+        z = np.uint64(key) + (np.arange(1, count + 1, dtype=np.uint64) + np.uint64(first)) * np.uint64(_GAMMA)
         z = (z ^ (z >> np.uint64(30))) * np.uint64(_M1)
         z = (z ^ (z >> np.uint64(27))) * np.uint64(_M2)
         return z ^ (z >> np.uint64(31))
@@ -150,3 +152,21 @@ def glorot_normal(key: Key, shape, dtype=np.float64) -> np.ndarray:
     receptive = math.prod(shape[:-2])
     fan_in, fan_out = shape[-2] * receptive, shape[-1] * receptive
     return _normal(key, shape, dtype, math.sqrt(2.0 / (fan_in + fan_out)), "glorot_normal")
+
+
+def dropout_mask(key: Key, shape, rate: float, counter: int = 0) -> np.ndarray:
+    """Truth values, True where dropout keeps an element: element e = counter + its row-major index takes the low
+    (even e) or high (odd e) half of word e // 2 of the key's stream and is kept when that is >= floor(rate * 2**32).
+    `qb200_dropout` and `qb200_dropout_layer_norm` draw the same mask on the device."""
+    rate = float(rate)
+    if not 0.0 <= rate < 1.0:
+        raise ValueError(f"dropout_mask requires a rate in [0, 1), got {rate}")
+    counter = operator.index(counter)
+    shape = _shape(shape)
+    count = math.prod(shape)
+    if not 0 <= counter <= _MASK - count:
+        raise ValueError(f"dropout_mask requires counter >= 0 and counter + {count} elements below 2**64, got {counter}")
+    odd = counter & 1
+    words = _stream(_key_value(key), (odd + count + 1) // 2, counter >> 1)
+    halves = np.stack((words & np.uint64(0xFFFFFFFF), words >> np.uint64(32)), axis=1).reshape(-1)
+    return (halves[odd:odd + count] >= np.uint64(math.floor(rate * 2.0**32))).reshape(shape)
