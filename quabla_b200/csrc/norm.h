@@ -50,6 +50,11 @@ struct DropoutArgs {
 
 // Elements of a row that one thread keeps in registers, and threads of a CTA at most.
 __host__ __device__ constexpr int norm_elements(size_t element_bytes) { return element_bytes == 8 ? 8 : 16; }
+// Rows that are on their way or in work in a thread's slots, and the bytes of the slots.
+__host__ __device__ constexpr int norm_stages(size_t element_bytes, int arrays) { return element_bytes >= 4 ? (arrays == 1 ? 4 : arrays == 2 ? 3 : 2) : 4; }
+constexpr size_t norm_ring_bytes(size_t element_bytes, int arrays) {
+    return norm_stages(element_bytes, arrays) * arrays * norm_elements(element_bytes) * element_bytes;
+}
 constexpr int NORM_MAX_THREADS = 512;
 constexpr int NORM_MAX_CLUSTER = 8;
 constexpr int NORM_SMS = 148;
