@@ -31,8 +31,8 @@ struct DrawStream {
         odd = (unsigned int)first & 1u;
         threshold = d.threshold;
     }
-    __device__ __forceinline__ unsigned long long word(unsigned long long j) const {
-        unsigned long long z = state + (j + 1) * 0x9e3779b97f4a7c15ull;
+    static constexpr unsigned long long GAMMA = 0x9e3779b97f4a7c15ull;
+    static __device__ __forceinline__ unsigned long long mix(unsigned long long z) {
         z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
         z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
         return z ^ (z >> 31);
@@ -40,22 +40,25 @@ struct DrawStream {
     // Keep decisions of the V consecutive elements from `index` (row-major, from 0) on.
     template <int V> __device__ __forceinline__ void keep(unsigned long long index, bool (&kept)[V]) const {
         const unsigned long long e = index + odd;
+        unsigned long long at = state + ((e >> 1) + 1) * GAMMA;  // of the word that holds e
         if constexpr (V == 1) {
-            const unsigned long long z = word(e >> 1);
+            const unsigned long long z = mix(at);
             kept[0] = ((e & 1) ? (unsigned int)(z >> 32) : (unsigned int)z) >= threshold;
         } else if ((e & 1) == 0) {
 #pragma unroll
             for (int j = 0; j < V; j += 2) {
-                const unsigned long long z = word((e >> 1) + j / 2);
+                const unsigned long long z = mix(at);
+                at += GAMMA;
                 kept[j] = (unsigned int)z >= threshold;
                 kept[j + 1] = (unsigned int)(z >> 32) >= threshold;
             }
         } else {
-            unsigned long long z = word(e >> 1);
+            unsigned long long z = mix(at);
 #pragma unroll
             for (int j = 0; j < V; j += 2) {
                 kept[j] = (unsigned int)(z >> 32) >= threshold;
-                z = word((e >> 1) + 1 + j / 2);
+                at += GAMMA;
+                z = mix(at);
                 kept[j + 1] = (unsigned int)z >= threshold;
             }
         }

@@ -129,7 +129,7 @@ qb200_status finish(const char* op, cudaError_t e) {
      : (dtype) == QB200_F16 ? qb::launch<__half>(args, stream)                      \
                             : qb::launch<__nv_bfloat16>(args, stream))
 
-qb::RowArray rows_of(const void* data, int64_t stride) { return {const_cast<void*>(data), (long long)stride}; }
+qb::RowArray rows_of(const void* data, int64_t stride) { return {const_cast<void*>(data), (long long)stride, 0}; }
 
 size_t workspace_bytes_for(int32_t dtype, int64_t rows, int32_t cols) {
     if (rows == 0) return 0;

@@ -11,7 +11,8 @@ namespace qb {
 
 struct RowArray {
     void* data = nullptr;
-    long long stride = 0;  // elements between rows
+    long long stride = 0;   // elements between rows
+    long long advance = 0;  // elements from a thread's row to its next one
 };
 
 struct NormForwardArgs {
