@@ -134,7 +134,7 @@ qb::RowArray rows_of(const void* data, int64_t stride) { return {const_cast<void
 size_t workspace_bytes_for(int32_t dtype, int64_t rows, int32_t cols) {
     if (rows == 0) return 0;
     const qb::RowShape s = qb::row_shape(cols, qb::norm_elements(element_bytes(dtype)));
-    return (size_t)qb::norm_partials(rows, s) * 2 * (size_t)cols * (dtype == QB200_F64 ? 8 : 4);
+    return (size_t)qb::norm_partials(rows, 1, s) * 2 * (size_t)cols * (dtype == QB200_F64 ? 8 : 4);
 }
 
 qb200_status run_forward(const char* op, int32_t dtype, int32_t param_dtype, qb::NormForwardArgs& a, const void* d_weight,

@@ -51,10 +51,27 @@ struct DropoutArgs {
 
 // Elements of a row that one thread keeps in registers, and threads of a CTA at most.
 __host__ __device__ constexpr int norm_elements(size_t element_bytes) { return element_bytes == 8 ? 8 : 16; }
-// Rows that are on their way or in work in a thread's slots, and the bytes of the slots.
-__host__ __device__ constexpr int norm_stages(size_t element_bytes, int arrays) { return element_bytes >= 4 ? (arrays == 1 ? 4 : arrays == 2 ? 3 : 2) : 4; }
-constexpr size_t norm_ring_bytes(size_t element_bytes, int arrays) {
-    return norm_stages(element_bytes, arrays) * arrays * norm_elements(element_bytes) * element_bytes;
+// Rows that a group works on at once.  16-bit rows that come 16 bytes at a time are bound by instruction issue: two
+// rows share a turn's reductions, barrier and addresses.
+__host__ __device__ constexpr int norm_forward_rows(size_t element_bytes, bool wide) { return element_bytes == 2 && wide ? 2 : 1; }
+__host__ __device__ constexpr int norm_backward_rows(size_t element_bytes, bool wide) { return element_bytes == 2 && wide ? 2 : 1; }
+// Whether the forward kernel's parameters are in shared memory instead of registers.
+__host__ __device__ constexpr bool norm_forward_shared_columns(size_t element_bytes, bool wide, bool residual) {
+    return element_bytes == 2 && wide && !residual;
+}
+// Turns whose rows are on their way or in work in a thread's slots.
+__host__ __device__ constexpr int norm_forward_stages(size_t element_bytes, bool wide, bool residual) {
+    return norm_forward_shared_columns(element_bytes, wide, residual) ? 2 : residual ? 3 : 4;
+}
+__host__ __device__ constexpr int norm_backward_stages(bool residual) { return residual ? 2 : 3; }
+// Shared memory of a thread: its slots, and its columns of weight and bias where they are there.
+constexpr size_t norm_forward_shared(size_t element_bytes, bool wide, bool residual) {
+    const size_t row = norm_elements(element_bytes) * element_bytes;
+    return norm_forward_stages(element_bytes, wide, residual) * norm_forward_rows(element_bytes, wide) * (residual ? 2 : 1) * row +
+           (norm_forward_shared_columns(element_bytes, wide, residual) ? 2 * norm_elements(element_bytes) * 4 : 0);
+}
+constexpr size_t norm_backward_shared(size_t element_bytes, bool wide, bool residual) {
+    return norm_backward_stages(residual) * norm_backward_rows(element_bytes, wide) * (residual ? 3 : 2) * norm_elements(element_bytes) * element_bytes;
 }
 constexpr int NORM_MAX_THREADS = 512;
 constexpr int NORM_MAX_CLUSTER = 8;
@@ -83,9 +100,10 @@ inline RowShape row_shape(int cols, int elements) {
     return s;
 }
 
-// Rows of partial weight gradients that a backward pass leaves (one per cluster of CTAs).
-inline int norm_partials(long long rows, const RowShape& s) {
-    const long long batches = (rows + s.groups - 1) / s.groups;
+// Rows of partial weight gradients that a backward pass leaves (one per cluster of CTAs); the most with one row at once.
+inline int norm_partials(long long rows, int rows_at_once, const RowShape& s) {
+    const int together = s.groups * rows_at_once;
+    const long long batches = (rows + together - 1) / together;
     const int resident = NORM_SMS * (s.threads_per_row * s.groups <= 256 ? 2 : 1) / s.cluster;
     return (int)(batches < resident ? batches : resident);
 }

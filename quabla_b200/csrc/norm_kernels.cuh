@@ -41,22 +41,28 @@ __device__ __forceinline__ double reciprocal_root(double v) { return 1.0 / sqrt(
 // otherwise be bound by instruction issue while 16-bit rows stream by.
 template <typename A> struct Two;
 template <> struct Two<float> {
-    float2 v;
+    unsigned long long v;  // the pair as the instructions take it
     __device__ __forceinline__ Two() {}
-    __device__ __forceinline__ Two(float a, float b) : v(make_float2(a, b)) {}
-    __device__ __forceinline__ explicit Two(float a) : v(make_float2(a, a)) {}
-    __device__ __forceinline__ float sum() const { return v.x + v.y; }
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+    __device__ __forceinline__ float2 both() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+    __device__ __forceinline__ float sum() const { const float2 f = both(); return f.x + f.y; }
 };
 template <> struct Two<double> {
     double2 v;
     __device__ __forceinline__ Two() {}
     __device__ __forceinline__ Two(double a, double b) : v(make_double2(a, b)) {}
     __device__ __forceinline__ explicit Two(double a) : v(make_double2(a, a)) {}
+    __device__ __forceinline__ double2 both() const { return v; }
     __device__ __forceinline__ double sum() const { return v.x + v.y; }
 };
-__device__ __forceinline__ Two<float> operator+(Two<float> a, Two<float> b) { a.v = __fadd2_rn(a.v, b.v); return a; }
-__device__ __forceinline__ Two<float> operator*(Two<float> a, Two<float> b) { a.v = __fmul2_rn(a.v, b.v); return a; }
-__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) { a.v = __ffma2_rn(a.v, b.v, c.v); return a; }
+__device__ __forceinline__ Two<float> operator+(Two<float> a, Two<float> b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
+__device__ __forceinline__ Two<float> operator*(Two<float> a, Two<float> b) { asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
+__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v)); return c; }
 __device__ __forceinline__ Two<double> operator+(Two<double> a, Two<double> b) { return {a.v.x + b.v.x, a.v.y + b.v.y}; }
 __device__ __forceinline__ Two<double> operator*(Two<double> a, Two<double> b) { return {a.v.x * b.v.x, a.v.y * b.v.y}; }
 __device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) { return {::fma(a.v.x, b.v.x, c.v.x), ::fma(a.v.y, b.v.y, c.v.y)}; }
@@ -65,69 +71,66 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 // A thread's packs of a row as pairs of accumulation-type values: pair q holds elements 2 q and 2 q + 1 of the packs
 // put one behind the other (of the same pack, or of two packs of one element).
-template <typename T, typename A>
-__device__ __forceinline__ T narrow_of(const Two<A>& p, int i) { return narrow<T>(i == 0 ? p.v.x : p.v.y); }
-
-template <typename T, int V, typename A>
-__device__ __forceinline__ void widen_pack(const Pack<T, V>& raw, Two<A>* pairs, int k) {
-    if constexpr (V == 1) {
-        (k % 2 == 0 ? pairs[k / 2].v.x : pairs[k / 2].v.y) = widen(raw.v[0]);
-    } else {
+template <typename T, int V, int K, typename A>
+__device__ __forceinline__ void widen_packs(const Pack<T, V> (&raw)[K], Two<A> (&pairs)[K * V / 2]) {
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            Two<A>& p = pairs[(k * V + i) / 2];
+    for (int q = 0; q < K * V / 2; ++q) {
+        if constexpr (V == 1) {
+            pairs[q] = Two<A>(widen(raw[2 * q].v[0]), widen(raw[2 * q + 1].v[0]));
+        } else {
+            const T* two = &raw[2 * q / V].v[2 * q % V];
             if constexpr (std::is_same<T, __half>::value) {
-                p.v = __half22float2(*reinterpret_cast<const __half2*>(&raw.v[i]));
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(two));
+                pairs[q] = Two<A>(f.x, f.y);
             } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // a bfloat16 is the upper half of a float32
-                const unsigned both = *reinterpret_cast<const unsigned*>(&raw.v[i]);
-                p.v.x = __uint_as_float(both << 16);
-                p.v.y = __uint_as_float(both & 0xffff0000u);
+                const unsigned u = *reinterpret_cast<const unsigned*>(two);
+                pairs[q] = Two<A>(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
             } else {
-                p.v.x = raw.v[i];
-                p.v.y = raw.v[i + 1];
+                pairs[q] = Two<A>(two[0], two[1]);
             }
         }
     }
 }
 
-template <typename T, int V, typename A>
-__device__ __forceinline__ Pack<T, V> narrow_pack(const Two<A>* pairs, int k) {
+template <typename T, int V, typename A, int H>
+__device__ __forceinline__ Pack<T, V> narrow_pack(const Two<A> (&pairs)[H], int k) {
     Pack<T, V> out;
     if constexpr (V == 1) {
-        out.v[0] = narrow_of<T>(pairs[k / 2], k % 2);
+        const auto f = pairs[k / 2].both();
+        out.v[0] = narrow<T>(k % 2 == 0 ? f.x : f.y);
     } else {
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
-            const Two<A>& p = pairs[(k * V + i) / 2];
-            if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(&out.v[i]) = __float22half2_rn(p.v);
-            else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(&out.v[i]) = __float22bfloat162_rn(p.v);
-            else out.v[i] = narrow<T>(p.v.x), out.v[i + 1] = narrow<T>(p.v.y);
+            const auto f = pairs[(k * V + i) / 2].both();
+            if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(&out.v[i]) = __float22half2_rn(f);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(&out.v[i]) = __float22bfloat162_rn(f);
+            else out.v[i] = narrow<T>(f.x), out.v[i + 1] = narrow<T>(f.y);
         }
     }
     return out;
 }
 
-// Columns [c, c + V) of a row, those at or behind `end` left as zero.
+// The first `count` elements of a pack.
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* row, int c, int end) {
+__device__ __forceinline__ Pack<T, V> load_pack(const T* from, int count) {
     Pack<T, V> p;
-    if (c + V <= end) {
-        p = *reinterpret_cast<const Pack<T, V>*>(row + c);
+    if (count >= V) {
+        p = *reinterpret_cast<const Pack<T, V>*>(from);
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) p.v[i] = c + i < end ? row[c + i] : narrow<T>((typename Accumulator<T>::type)0);
+        for (int i = 0; i < V; ++i) p.v[i] = i < count ? from[i] : narrow<T>((typename Accumulator<T>::type)0);
     }
     return p;
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void store_pack(T* row, int c, int end, const Pack<T, V>& p) {
-    if (c + V <= end) {
-        *reinterpret_cast<Pack<T, V>*>(row + c) = p;
+__device__ __forceinline__ void store_pack(T* to, int count, const Pack<T, V>& p) {
+    if (count >= V) {
+        *reinterpret_cast<Pack<T, V>*>(to) = p;
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (c + i < end) row[c + i] = p.v[i];
+            if (i < count) to[i] = p.v[i];
     }
 }
 
@@ -136,51 +139,114 @@ __device__ __forceinline__ A load_param(const void* params, bool f32, int c) {
     return f32 ? (A) static_cast<const float*>(params)[c] : (A)widen(static_cast<const T*>(params)[c]);
 }
 
-// Sums over the threads of a row, the same in every one of them: shuffles within a warp, shared memory across the
+// How a thread finds its place.  SPAN is 32 where a row has one or more whole warps, each with 32 * E columns of its own
+// one behind the other; 0 where several rows share a warp (threads_per_row is then a power of two below 32).  Pack k of a
+// thread starts at column `at` + k * hop.  With whole warps every distance within a thread's packs and slots is a
+// constant of the instruction: with distances from the launch instead the kernels issued half as many instructions again.
+template <typename T, int V, int SPAN, int ROWS> struct Place {
+    static constexpr int E = norm_elements(sizeof(T)), K = E / V;
+    int t, group, rank, begin, end, at;
+    int run_hop;
+    int there[ROWS];     // turns in which row r of the group exists
+    int step;            // rows from one turn to the next
+    long long row;       // the group works on rows [row, row + ROWS) at once
+    __device__ __forceinline__ Place(const RowShape& shape, int cols, long long rows) {
+        const int span = SPAN == 32 ? 32 : shape.threads_per_row;
+        t = threadIdx.x % shape.threads_per_row;
+        group = threadIdx.x / shape.threads_per_row;
+        rank = blockIdx.x % shape.cluster;
+        begin = rank * shape.slice;
+        end = begin + shape.slice < cols ? begin + shape.slice : cols;
+        at = begin + t / span * span * E + t % span * V;
+        run_hop = span * V;
+        step = (int)(gridDim.x / shape.cluster) * shape.groups * ROWS;
+        row = ((long long)(blockIdx.x / shape.cluster) * shape.groups + group) * ROWS;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) there[r] = row + r < rows ? (int)((rows - row - r + step - 1) / step) : 0;
+    }
+    // Turns of the whole CTA and cluster: those of group 0's first row, whose barriers all take part in.
+    __device__ __forceinline__ int turns(long long rows) const {
+        const long long first = row - group * ROWS;
+        return first < rows ? (int)((rows - first + step - 1) / step) : 0;
+    }
+    __device__ __forceinline__ int hop() const { return SPAN == 32 ? 32 * V : run_hop; }
+    // Elements of pack k that are in the row.
+    __device__ __forceinline__ int count(int k) const {
+        const int left = end - at - k * hop();
+        return left >= V ? V : left > 0 ? left : 0;
+    }
+    __device__ __forceinline__ bool whole() const { return at + (K - 1) * hop() + V <= end; }
+    template <typename A>
+    __device__ __forceinline__ void store(T* row_at, const Two<A> (&pairs)[E / 2], bool all) const {
+        if (all) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) *reinterpret_cast<Pack<T, V>*>(row_at + k * hop()) = narrow_pack<T, V>(pairs, k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) store_pack<T, V>(row_at + k * hop(), count(k), narrow_pack<T, V>(pairs, k));
+        }
+    }
+};
+
+// N sums over the threads of a row, the same in every one of them: shuffles within a warp, shared memory across the
 // warps of the row's group (a named barrier for each group, so groups do not wait for one another), distributed shared
-// memory across the CTAs of a cluster.  Two buffers in turn, so each sum costs one barrier at each level.
-template <typename A, int N> struct RowSum {
+// memory across the CTAs of a cluster.  Two buffers in turn, so each call costs one barrier at each level.
+template <typename A, int N, int SPAN> struct RowSum {
+    static constexpr int LANES = 32 / N;  // that carry one of the sums on
     struct Shared {
-        A warps[2][2][NORM_MAX_THREADS / 32];
+        A warps[2][N][NORM_MAX_THREADS / 32];
         A ranks[2][NORM_MAX_CLUSTER][N];
     };
     Shared& shared;
-    const int threads_per_row;
-    const int cluster;
+    const int threads_per_row, cluster, lane, warp, warps, group;
     int turn = 0;
-    __device__ RowSum(Shared& s, int t, int c) : shared(s), threads_per_row(t), cluster(c) {}
-
-    // Over the lanes of one row in a warp; every lane has the sums.
-    __device__ __forceinline__ void across(A (&v)[N]) const {
-        for (int offset = threads_per_row / 2; offset > 0; offset /= 2)
-#pragma unroll
-            for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], offset);
-    }
+    __device__ __forceinline__ RowSum(Shared& s, const RowShape& shape)
+        : shared(s), threads_per_row(shape.threads_per_row), cluster(shape.cluster), lane(threadIdx.x % 32), warp(threadIdx.x / 32),
+          warps(shape.threads_per_row / 32), group(threadIdx.x / shape.threads_per_row) {}
 
     __device__ __forceinline__ void operator()(A (&v)[N]) {
-        if (threads_per_row < 32) return across(v);
-        // Over the warp.  Of two sums, one half of the lanes goes on with the first and the other with the second.
-        const int lane = threadIdx.x % 32;
-        A part = v[0];
-        if (N == 2) {
-            const A send = lane < 16 ? v[N - 1] : v[0];
-            part = (lane < 16 ? v[0] : v[N - 1]) + __shfl_xor_sync(0xffffffffu, send, 16);
+        if constexpr (SPAN == 32) {
+            whole_warps(v);
         } else {
-            part += __shfl_xor_sync(0xffffffffu, part, 16);
-        }
+            for (int offset = threads_per_row / 2; offset > 0; offset /= 2)
 #pragma unroll
-        for (int offset = 8; offset > 0; offset /= 2) part += __shfl_xor_sync(0xffffffffu, part, offset);
-        if (threads_per_row > 32) {
-            // Over the (at most 16) warps of the row: lane l adds up from warp l % 16 on.
-            const int warp = threadIdx.x / 32, warps = threads_per_row / 32, group = warp / warps, first = group * warps;
-            if (lane % 16 == 0) shared.warps[turn][lane / 16][warp] = part;
+                for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], offset);
+        }
+    }
+
+private:
+    __device__ __forceinline__ void whole_warps(A (&v)[N]) {
+        // Over the warp.  While there are several sums, half of the lanes goes on with half of them: lanes
+        // [n * LANES, (n + 1) * LANES) end up with sum n.
+        A part[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) part[n] = v[n];
+#pragma unroll
+        for (int offset = 16, left = N; offset > 0; offset /= 2) {
+            if (left > 1) {
+                left /= 2;
+#pragma unroll
+                for (int n = 0; n < left; ++n) {
+                    const A send = lane & offset ? part[n] : part[n + left];
+                    part[n] = (lane & offset ? part[n + left] : part[n]) + __shfl_xor_sync(0xffffffffu, send, offset);
+                }
+            } else {
+                part[0] += __shfl_xor_sync(0xffffffffu, part[0], offset);
+            }
+        }
+        if (warps > 1) {  // over the (at most 16) warps of the row
+            A* const here = shared.warps[turn][lane / LANES];
+            if (lane % LANES == 0) here[warp] = part[0];
             asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads_per_row) : "memory");  // 0 is the whole CTA's
-            part = lane % 16 < warps ? shared.warps[turn][lane / 16][first + lane % 16] : (A)0;
+            constexpr int PART = LANES < 16 ? LANES : 16;
+            const A* const there = here + group * warps;
+            part[0] = lane % PART < warps ? there[lane % PART] : (A)0;
+            if (PART < 16 && lane % PART + PART < warps) part[0] += there[lane % PART + PART];
 #pragma unroll
-            for (int offset = 8; offset > 0; offset /= 2) part += __shfl_xor_sync(0xffffffffu, part, offset);
+            for (int offset = PART / 2; offset > 0; offset /= 2) part[0] += __shfl_xor_sync(0xffffffffu, part[0], offset);
         }
-        v[0] = N == 2 ? __shfl_sync(0xffffffffu, part, 0) : part;
-        if (N == 2) v[N - 1] = __shfl_sync(0xffffffffu, part, 16);
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = N == 1 ? part[0] : __shfl_sync(0xffffffffu, part[0], n * LANES);
         if (cluster > 1) {
             auto c = cooperative_groups::this_cluster();
             if ((int)threadIdx.x < cluster) {
@@ -200,194 +266,237 @@ template <typename A, int N> struct RowSum {
 };
 
 // Rows on their way in: every thread copies the packs that it will work on itself (cp.async into slots of its own), a
-// few rows ahead of the one in work, so the copies need no barrier and their latency is hidden whatever the occupancy.
-// Packs behind a row's end or the last row arrive as zeros.
-// Slot s of neighbouring threads lie next to each other: one warp's copy is one run of shared memory (with a thread's
-// slots together instead, the same kernels took 10 to 35 % longer).
-template <typename T, int V, int ARRAYS, int STAGES> struct RowRing {
+// few turns ahead of the one in work, so the copies need no barrier and their latency is hidden whatever the occupancy.
+// Packs behind a row's end or the last row arrive as zeros.  The same slot of a warp's lanes is one run of shared memory
+// (with a thread's slots together instead, the kernels took 10 to 35 % longer).
+template <typename T, int V, int ARRAYS, int ROWS, int STAGES> struct RowRing {
     static constexpr int E = norm_elements(sizeof(T)), K = E / V, BYTES = V * sizeof(T);
-    char* const slots;   // [STAGES][ARRAYS][K][threads]
-    const int pitch;     // bytes from one slot of a thread to its next
-    __device__ explicit RowRing(void* shared)
-        : slots(static_cast<char*>(shared) + threadIdx.x * BYTES), pitch((int)blockDim.x * BYTES) {}
-    __device__ __forceinline__ Pack<T, V>* at(int stage, int array, int k) const {
-        return reinterpret_cast<Pack<T, V>*>(slots + (stage * (ARRAYS * K) + array * K + k) * pitch);
+    static constexpr int STAGE_BYTES = ROWS * ARRAYS * K * 32 * BYTES;  // of a warp
+    static constexpr int THREAD_BYTES = STAGES * ROWS * ARRAYS * E * sizeof(T);
+    char* const slots;  // [warps][STAGES][ROWS][ARRAYS][K][32]
+    __device__ __forceinline__ explicit RowRing(void* shared)
+        : slots(static_cast<char*>(shared) + threadIdx.x / 32 * (STAGES * STAGE_BYTES) + threadIdx.x % 32 * BYTES) {}
+    __device__ __forceinline__ char* stage(int s) const { return slots + s * STAGE_BYTES; }
+    static __device__ __forceinline__ Pack<T, V>* at(char* stage, int r, int array, int k) {
+        return reinterpret_cast<Pack<T, V>*>(stage + ((r * ARRAYS + array) * K + k) * 32 * BYTES);
+    }
+    static __device__ __forceinline__ void fetch(char* stage, int r, int array, int k, const T* from) {
+        if constexpr (BYTES >= 4) {
+            const unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, r, array, k));
+            if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+            else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES < 4 ? 4 : BYTES) : "memory");
+        } else {
+            at(stage, r, array, k)->v[0] = *from;
+        }
     }
     // `count` elements at `from`: a whole pack, less at a row's end, none for a row that is not there.
-    __device__ __forceinline__ void fetch(int stage, int array, int k, const T* from, int count) const {
-        Pack<T, V>* slot = at(stage, array, k);
+    static __device__ __forceinline__ void fetch(char* stage, int r, int array, int k, const T* from, int count) {
         if constexpr (BYTES >= 4) {
-            const unsigned to = (unsigned)__cvta_generic_to_shared(slot);
+            const unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, r, array, k));
             const int bytes = count * (int)sizeof(T);
             if constexpr (BYTES == 16)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
             else
                 asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES < 4 ? 4 : BYTES), "r"(bytes) : "memory");
         } else {
-            slot->v[0] = count > 0 ? *from : narrow<T>((typename Accumulator<T>::type)0);
+            at(stage, r, array, k)->v[0] = count > 0 ? *from : narrow<T>((typename Accumulator<T>::type)0);
         }
     }
     // A thread's packs of a row as pairs.
-    template <typename A> __device__ __forceinline__ void read(int stage, int array, Two<A> (&pairs)[E / 2]) const {
+    template <typename A> static __device__ __forceinline__ void read(char* stage, int r, int array, Two<A> (&pairs)[E / 2]) {
+        Pack<T, V> raw[K];
 #pragma unroll
-        for (int k = 0; k < K; ++k) widen_pack<T, V>(*at(stage, array, k), pairs, k);
+        for (int k = 0; k < K; ++k) raw[k] = *at(stage, r, array, k);
+        widen_packs<T, V>(raw, pairs);
     }
     static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-    // All but the youngest STAGES - 1 batches of copies have landed.
+    // All but the youngest STAGES - 1 turns' copies have landed.
     static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory"); }
 };
 
-// A kernel's place in the rows: which columns a thread holds, and which row its group is at.
-template <typename T, int V> struct Place {
-    static constexpr int E = norm_elements(sizeof(T)), K = E / V;
-    int t, group, rank, begin, end, at, hop;
-    long long step, row;
-    __device__ __forceinline__ Place(const RowShape& shape, int cols) {
-        t = threadIdx.x % shape.threads_per_row;
-        group = threadIdx.x / shape.threads_per_row;
-        rank = blockIdx.x % shape.cluster;
-        begin = rank * shape.slice;
-        end = begin + shape.slice < cols ? begin + shape.slice : cols;
-        at = begin + t * V;  // pack k: columns from at + k * hop on
-        hop = shape.threads_per_row * V;
-        step = (long long)(gridDim.x / shape.cluster) * shape.groups;
-        row = (long long)(blockIdx.x / shape.cluster) * shape.groups + group;
+// A thread's columns of a parameter, 1 or 0 where there is none: in registers, or in slots of its own in shared memory
+// where registers are worth more.
+template <typename T, int V, bool SHARED> struct Columns {
+    using A = typename Accumulator<T>::type;
+    static constexpr int E = norm_elements(sizeof(T)), H = E / 2, W = 16 / sizeof(Two<A>);
+    struct alignas(16) Slot { Two<A> v[W]; };
+    static constexpr int THREAD_BYTES = SHARED ? E * sizeof(A) : 0;
+    Two<A> pairs[SHARED ? 1 : H];
+    Slot* slots;  // [warps][H / W][32]
+    template <typename P>
+    __device__ __forceinline__ Columns(const P& place, const void* params, bool f32, A absent, char* shared) {
+        slots = reinterpret_cast<Slot*>(shared) + threadIdx.x / 32 * (H / W * 32) + threadIdx.x % 32;
+#pragma unroll
+        for (int q = 0; q < H; ++q) {
+            A v[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int c = place.at + (2 * q + i) / V * place.hop() + (2 * q + i) % V;
+                v[i] = params != nullptr && c < place.end ? load_param<T, A>(params, f32, c) : absent;
+            }
+            if constexpr (SHARED) slots[q / W * 32].v[q % W] = Two<A>(v[0], v[1]);
+            else pairs[q] = Two<A>(v[0], v[1]);
+        }
     }
-    // Elements of pack k that are in the row.
-    __device__ __forceinline__ int count(int k) const {
-        const int left = end - at - k * hop;
-        return left >= V ? V : left > 0 ? left : 0;
-    }
-    __device__ __forceinline__ bool whole() const { return at + (K - 1) * hop + V <= end; }
-    __device__ __forceinline__ void store(T* row_at, int k, const Pack<T, V>& pack, bool all) const {
-        if (all) *reinterpret_cast<Pack<T, V>*>(row_at + k * hop) = pack;
-        else store_pack<T, V>(row_at + k * hop, 0, count(k), pack);
+    __device__ __forceinline__ void get(Two<A> (&out)[H]) const {
+        if constexpr (SHARED) {
+#pragma unroll
+            for (int w = 0; w < H / W; ++w) {
+                const Slot slot = slots[w * 32];
+#pragma unroll
+                for (int i = 0; i < W; ++i) out[w * W + i] = slot.v[i];
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < H; ++q) out[q] = pairs[q];
+        }
     }
 };
 
-// Adds scale or 0 by the elements' draws: pairs of pack k, whose first element has row-major number `index`.
-template <int V, typename A>
-__device__ __forceinline__ void drop(const DrawStream& draws, unsigned long long index, A scale, Two<A>* pairs, int k) {
-    bool keep[V];
-    draws.keep(index, keep);
+// Dropout of a thread's packs of a row; `index` is the row-major number of its first column.
+template <int V, typename A, int H>
+__device__ __forceinline__ void drop(const DrawStream& draws, unsigned long long index, int hop, A scale, Two<A> (&pairs)[H]) {
+    constexpr int K = 2 * H / V;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        A& v = (k * V + i) % 2 == 0 ? pairs[(k * V + i) / 2].v.x : pairs[(k * V + i) / 2].v.y;
-        v = keep[i] ? v * scale : (A)0;
+    for (int k = 0; k < K; ++k) {
+        bool keep[V];
+        draws.keep(index + k * hop, keep);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            Two<A>& pair = pairs[(k * V + i) / 2];
+            const auto f = pair.both();
+            if (V == 1) pair = k % 2 == 0 ? Two<A>(keep[0] ? f.x * scale : (A)0, f.y) : Two<A>(f.x, keep[0] ? f.y * scale : (A)0);
+            else if (i % 2 == 0) pair = Two<A>(keep[i] ? f.x * scale : (A)0, keep[(i + 1) % V] ? f.y * scale : (A)0);
+        }
     }
 }
 
 // RESIDUAL: x passes through dropout and may be added to a residual; otherwise h = x.
-template <typename T, int V, bool RESIDUAL>
-__global__ void __launch_bounds__(NORM_MAX_THREADS)
+template <typename T, int V, int SPAN, bool RESIDUAL>
+__global__ void __maxnreg__(128)
 norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
-    constexpr int ARRAYS = RESIDUAL ? 2 : 1, STAGES = norm_stages(sizeof(T), ARRAYS);
-    using Ring = RowRing<T, V, ARRAYS, STAGES>;
+    constexpr int ARRAYS = RESIDUAL ? 2 : 1, R = norm_forward_rows(sizeof(T), V > 1), STAGES = norm_forward_stages(sizeof(T), V > 1, RESIDUAL);
+    constexpr bool SHARED = norm_forward_shared_columns(sizeof(T), V > 1, RESIDUAL);
+    using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
-    __shared__ typename RowSum<A, 1>::Shared shared;
-    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ typename RowSum<A, R, SPAN>::Shared shared;
+    extern __shared__ __align__(16) char dynamic[];
     const Ring ring(dynamic);
-    RowSum<A, 1> row_sum(shared, shape.threads_per_row, shape.cluster);
-    const Place<T, V> place(shape, p.cols);
-    const bool whole = place.whole();
-    long long row = place.row, ahead = place.row;
-    const bool added = RESIDUAL && p.residual.data != nullptr;
+    RowSum<A, R, SPAN> row_sum(shared, shape);
+    const Place<T, V, SPAN, R> place(shape, p.cols, p.rows);
+    const bool whole = place.whole(), added = RESIDUAL && p.residual.data != nullptr;
+    long long row = place.row;
     const T* x = static_cast<const T*>(p.x.data) + row * p.x.stride + place.at;
     const T* residual = static_cast<const T*>(p.residual.data) + row * p.residual.stride + place.at;
     T* h_out = static_cast<T*>(p.h.data) + row * p.h.stride + place.at;
     T* y = static_cast<T*>(p.y.data) + row * p.y.stride + place.at;
 
-    auto fetch = [&](int stage) {
-        const bool there = ahead < p.rows;
+    auto fetch = [&](char* stage, int turn) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int count = there ? (whole ? V : place.count(k)) : 0;
-            ring.fetch(stage, 0, k, x + k * place.hop, count);
-            if (added) ring.fetch(stage, ARRAYS - 1, k, residual + k * place.hop, count);
+        for (int r = 0; r < R; ++r) {
+            const T* from = x + r * p.x.stride;
+            const T* more = residual + r * p.residual.stride;
+            if (whole && turn < place.there[r]) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    ring.fetch(stage, r, 0, k, from + k * place.hop());
+                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, more + k * place.hop());
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const int count = turn < place.there[r] ? place.count(k) : 0;
+                    ring.fetch(stage, r, 0, k, from + k * place.hop(), count);
+                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, more + k * place.hop(), count);
+                }
+            }
         }
         ring.commit();
-        ahead += place.step;
         x += p.x.advance;
-        residual += p.residual.advance;
+        if (RESIDUAL) residual += p.residual.advance;
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch(s);
+    for (int s = 0; s < STAGES - 1; ++s) fetch(ring.stage(s), s);
 
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale, inverse = (A)1 / (A)p.cols;
-    Two<A> weight[E / 2], bias[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = place.at + e / V * place.hop + e % V;
-        const A w = p.weight != nullptr && c < place.end ? load_param<T, A>(p.weight, p.params_f32, c) : (A)1;
-        const A b = p.bias != nullptr && c < place.end ? load_param<T, A>(p.bias, p.params_f32, c) : (A)0;
-        (e % 2 == 0 ? weight[e / 2].v.x : weight[e / 2].v.y) = w;
-        (e % 2 == 0 ? bias[e / 2].v.x : bias[e / 2].v.y) = b;
-    }
+    using Cols = Columns<T, V, SHARED>;
+    char* const behind = dynamic + Ring::THREAD_BYTES * blockDim.x;
+    const Cols weights(place, p.weight, p.params_f32, (A)1, behind);
+    const Cols biases(place, p.bias, p.params_f32, (A)0, behind + Cols::THREAD_BYTES * blockDim.x);
 
-    // The groups of a CTA and the CTAs of a cluster make the same number of turns: `first` is that of group 0.
-    int stage = 0;
-    for (long long first = row - place.group; first < p.rows; first += place.step) {
-        fetch(stage == 0 ? STAGES - 1 : stage - 1);  // into the slots that were read in the last turn
+    const int turns = place.turns(p.rows);
+    char *now = ring.stage(0), *free = ring.stage(STAGES - 1);  // the slots in work; those read in the last turn
+    for (int turn = 0; turn < turns; ++turn) {
+        fetch(free, turn + STAGES - 1);
         ring.wait();
-        const bool live = row < p.rows;
-        Two<A> h[E / 2];
-        ring.read(stage, 0, h);
-        if (RESIDUAL) {
-            if (p.draw.threshold != 0)
+        Two<A> h[R][E / 2];
+        A sum[R];
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    drop<V>(draws, (unsigned long long)row * p.cols + place.at + k * place.hop, scale, h, k);
-            if (added) {
-                Two<A> more[E / 2];
-                ring.read(stage, ARRAYS - 1, more);
+        for (int r = 0; r < R; ++r) {
+            ring.read(now, r, 0, h[r]);
+            if (RESIDUAL) {
+                if (p.draw.threshold != 0) drop<V>(draws, (unsigned long long)(row + r) * p.cols + place.at, place.hop(), scale, h[r]);
+                if (added) {
+                    Two<A> more[E / 2];
+                    ring.read(now, r, ARRAYS - 1, more);
 #pragma unroll
-                for (int q = 0; q < E / 2; ++q) h[q] = h[q] + more[q];
-            }
-            if (p.h.data != nullptr && live)
-#pragma unroll
-                for (int k = 0; k < K; ++k) place.store(h_out, k, narrow_pack<T, V>(h, k), whole);
-        }
-        Two<A> total = h[0];
-#pragma unroll
-        for (int q = 1; q < E / 2; ++q) total = total + h[q];
-        A sum[1] = {total.sum()};
-        row_sum(sum);
-        const A mean = sum[0] * inverse;
-        Two<A> spread((A)0);
-#pragma unroll
-        for (int q = 0; q < E / 2; ++q) h[q] = h[q] + Two<A>(-mean);
-        if (whole) {
-#pragma unroll
-            for (int q = 0; q < E / 2; ++q) spread = fma(h[q], h[q], spread);
-        } else {  // what lies behind the row's end does not count
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const Two<A>& d = h[(k * V + i) / 2];
-                    const A v = (k * V + i) % 2 == 0 ? d.v.x : d.v.y;
-                    if (i < place.count(k)) spread.v.x += v * v;
+                    for (int q = 0; q < E / 2; ++q) h[r][q] = h[r][q] + more[q];
                 }
+                if (p.h.data != nullptr && turn < place.there[r]) place.store(h_out + r * p.h.stride, h[r], whole);
+            }
+            Two<A> even = h[r][0], odd = h[r][1];
+#pragma unroll
+            for (int q = 2; q < E / 2; q += 2) even = even + h[r][q], odd = odd + h[r][q + 1];
+            sum[r] = (even + odd).sum();
         }
-        A squares[1] = {spread.sum()};
+        free = now;
+        now = now == ring.stage(STAGES - 1) ? ring.stage(0) : now + Ring::STAGE_BYTES;
+        row_sum(sum);
+        A squares[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            sum[r] *= inverse;
+            const Two<A> away(-sum[r]);
+#pragma unroll
+            for (int q = 0; q < E / 2; ++q) h[r][q] = h[r][q] + away;
+            if (whole) {
+                Two<A> even = h[r][0] * h[r][0], odd = h[r][1] * h[r][1];
+#pragma unroll
+                for (int q = 2; q < E / 2; q += 2) even = fma(h[r][q], h[r][q], even), odd = fma(h[r][q + 1], h[r][q + 1], odd);
+                squares[r] = (even + odd).sum();
+            } else {  // what lies behind the row's end does not count
+                squares[r] = (A)0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const auto d = h[r][e / 2].both();
+                    const A v = e % 2 == 0 ? d.x : d.y;
+                    if (e % V < place.count(e / V)) squares[r] += v * v;
+                }
+            }
+        }
         row_sum(squares);
-        const A rstd = reciprocal_root(squares[0] * inverse + (A)p.epsilon);
+        Two<A> weight[E / 2], bias[E / 2];
+        weights.get(weight);
+        biases.get(bias);
 #pragma unroll
-        for (int q = 0; q < E / 2; ++q) h[q] = fma(h[q] * Two<A>(rstd), weight[q], bias[q]);
-        if (live) {
+        for (int r = 0; r < R; ++r) {
+            const A rstd = reciprocal_root(squares[r] * inverse + (A)p.epsilon);
+            const Two<A> factor(rstd);
 #pragma unroll
-            for (int k = 0; k < K; ++k) place.store(y, k, narrow_pack<T, V>(h, k), whole);
-            if (place.t == 0 && place.rank == 0) {
-                if (p.mean != nullptr) static_cast<A*>(p.mean)[row] = mean;
-                if (p.rstd != nullptr) static_cast<A*>(p.rstd)[row] = rstd;
+            for (int q = 0; q < E / 2; ++q) h[r][q] = fma(h[r][q] * factor, weight[q], bias[q]);
+            if (turn < place.there[r]) {
+                place.store(y + r * p.y.stride, h[r], whole);
+                if (place.t == 0 && place.rank == 0) {
+                    if (p.mean != nullptr) static_cast<A*>(p.mean)[row + r] = sum[r];
+                    if (p.rstd != nullptr) static_cast<A*>(p.rstd)[row + r] = rstd;
+                }
             }
         }
         row += place.step;
-        h_out += p.h.advance;
         y += p.y.advance;
-        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        if (RESIDUAL) h_out += p.h.advance;
     }
 }
 
@@ -402,117 +511,134 @@ __device__ __forceinline__ void store_gradient(void* out, bool f32, int c, A v) 
 // Threads keep their columns' share of dweight and dbias in registers over all rows of the CTA; at the end the CTA's
 // groups are added up through shared memory, in order, and the CTA writes one row of partial sums (the gradients
 // themselves where there is only one).
-template <typename T, int V, bool RESIDUAL>
-__global__ void __launch_bounds__(NORM_MAX_THREADS)
+template <typename T, int V, int SPAN, bool RESIDUAL>
+__global__ void __maxnreg__(128)
 norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
-    constexpr int ARRAYS = RESIDUAL ? 3 : 2, STAGES = norm_stages(sizeof(T), ARRAYS);
-    using Ring = RowRing<T, V, ARRAYS, STAGES>;
+    constexpr int ARRAYS = RESIDUAL ? 3 : 2, R = norm_backward_rows(sizeof(T), V > 1), STAGES = norm_backward_stages(RESIDUAL);
+    using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
-    __shared__ typename RowSum<A, 2>::Shared shared;
-    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ typename RowSum<A, 2 * R, SPAN>::Shared shared;
+    extern __shared__ __align__(16) char dynamic[];
     const Ring ring(dynamic);
-    RowSum<A, 2> row_sum(shared, shape.threads_per_row, shape.cluster);
-    const Place<T, V> place(shape, p.cols);
-    const bool whole = place.whole();
-    long long row = place.row, ahead = place.row;
-    const bool added = RESIDUAL && p.dh.data != nullptr;
+    RowSum<A, 2 * R, SPAN> row_sum(shared, shape);
+    const Place<T, V, SPAN, R> place(shape, p.cols, p.rows);
+    const bool whole = place.whole(), added = RESIDUAL && p.dh.data != nullptr;
+    long long row = place.row;
     const T* dy = static_cast<const T*>(p.dy.data) + row * p.dy.stride + place.at;
     const T* h = static_cast<const T*>(p.h.data) + row * p.h.stride + place.at;
     const T* dh = static_cast<const T*>(p.dh.data) + row * p.dh.stride + place.at;
     T* dx = static_cast<T*>(p.dx.data) + row * p.dx.stride + place.at;
     T* dresidual = static_cast<T*>(p.dresidual.data) + row * p.dresidual.stride + place.at;
 
-    auto fetch = [&](int stage) {
-        const bool there = ahead < p.rows;
+    auto fetch = [&](char* stage, int turn) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int count = there ? (whole ? V : place.count(k)) : 0;
-            ring.fetch(stage, 0, k, dy + k * place.hop, count);
-            ring.fetch(stage, 1, k, h + k * place.hop, count);
-            if (added) ring.fetch(stage, ARRAYS - 1, k, dh + k * place.hop, count);
+        for (int r = 0; r < R; ++r) {
+            const T* from[3] = {dy + r * p.dy.stride, h + r * p.h.stride, dh + r * p.dh.stride};
+            if (whole && turn < place.there[r]) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    ring.fetch(stage, r, 0, k, from[0] + k * place.hop());
+                    ring.fetch(stage, r, 1, k, from[1] + k * place.hop());
+                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, from[2] + k * place.hop());
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const int count = turn < place.there[r] ? place.count(k) : 0;
+                    ring.fetch(stage, r, 0, k, from[0] + k * place.hop(), count);
+                    ring.fetch(stage, r, 1, k, from[1] + k * place.hop(), count);
+                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, from[2] + k * place.hop(), count);
+                }
+            }
         }
         ring.commit();
-        ahead += place.step;
         dy += p.dy.advance;
         h += p.h.advance;
-        dh += p.dh.advance;
+        if (RESIDUAL) dh += p.dh.advance;
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch(s);
+    for (int s = 0; s < STAGES - 1; ++s) fetch(ring.stage(s), s);
 
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale, inverse = (A)1 / (A)p.cols;
-    Two<A> weight[E / 2], dweight[E / 2], dbias[E / 2];
+    const Columns<T, V, false> weights(place, p.weight, p.params_f32, (A)1, dynamic);
+    const auto& weight = weights.pairs;
+    Two<A> dweight[E / 2], dbias[E / 2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = place.at + e / V * place.hop + e % V;
-        (e % 2 == 0 ? weight[e / 2].v.x : weight[e / 2].v.y) =
-            p.weight != nullptr && c < place.end ? load_param<T, A>(p.weight, p.params_f32, c) : (A)1;
-        dweight[e / 2] = dbias[e / 2] = Two<A>((A)0);
-    }
+    for (int q = 0; q < E / 2; ++q) dweight[q] = dbias[q] = Two<A>((A)0);
 
-    const A* means = static_cast<const A*>(p.mean);
-    const A* rstds = static_cast<const A*>(p.rstd);
-    A next_mean = row < p.rows ? means[row] : (A)0, next_rstd = row < p.rows ? rstds[row] : (A)0;
-    int stage = 0;
-    for (long long first = row - place.group; first < p.rows; first += place.step) {
-        fetch(stage == 0 ? STAGES - 1 : stage - 1);
-        const Two<A> away(-next_mean), rstd(next_rstd);
-        if (row + place.step < p.rows) {
-            next_mean = means[row + place.step];
-            next_rstd = rstds[row + place.step];
+    const A* means = static_cast<const A*>(p.mean) + row;
+    const A* rstds = static_cast<const A*>(p.rstd) + row;
+    A next_mean[R], next_rstd[R];
+    auto fetch_statistics = [&](int turn) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            next_mean[r] = turn < place.there[r] ? means[r] : (A)0;
+            next_rstd[r] = turn < place.there[r] ? rstds[r] : (A)0;
         }
+        means += place.step;
+        rstds += place.step;
+    };
+    fetch_statistics(0);
+    const int turns = place.turns(p.rows);
+    char *now = ring.stage(0), *free = ring.stage(STAGES - 1);
+    for (int turn = 0; turn < turns; ++turn) {
+        fetch(free, turn + STAGES - 1);
+        Two<A> away[R], rstd[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            away[r] = Two<A>(-next_mean[r]);
+            rstd[r] = Two<A>(next_rstd[r]);
+        }
+        fetch_statistics(turn + 1);
         ring.wait();
-        Two<A> one((A)0), along((A)0);
-        {
-            Two<A> d[E / 2], normal[E / 2];
-            ring.read(stage, 0, d);
-            ring.read(stage, 1, normal);
+        A sums[2 * R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            Two<A> d[E / 2], normal[E / 2], one((A)0), along((A)0);
+            ring.read(now, r, 0, d);
+            ring.read(now, r, 1, normal);
 #pragma unroll
             for (int q = 0; q < E / 2; ++q) {
-                normal[q] = (normal[q] + away) * rstd;
+                normal[q] = (normal[q] + away[r]) * rstd[r];
                 const Two<A> g = d[q] * weight[q];
                 dweight[q] = fma(d[q], normal[q], dweight[q]);
                 dbias[q] = dbias[q] + d[q];
                 one = one + g;
                 along = fma(g, normal[q], along);
             }
+            sums[2 * r] = one.sum();
+            sums[2 * r + 1] = along.sum();
         }
-        A sums[2] = {one.sum(), along.sum()};
         row_sum(sums);
-        const Two<A> along_one(-sums[0] * inverse), along_normal(-sums[1] * inverse);
-        // The row is read from its slots once more: the registers hold the parameters' gradients.
-        Two<A> d[E / 2], normal[E / 2];
-        ring.read(stage, 0, d);
-        ring.read(stage, 1, normal);
+        // The rows are read from their slots once more: the registers hold the parameters' gradients.
 #pragma unroll
-        for (int q = 0; q < E / 2; ++q) {
-            normal[q] = (normal[q] + away) * rstd;
-            d[q] = rstd * (fma(d[q], weight[q], along_one) + normal[q] * along_normal);
-        }
-        const bool live = row < p.rows;
-        if (RESIDUAL) {
-            if (added) {
-                ring.read(stage, ARRAYS - 1, normal);
+        for (int r = 0; r < R; ++r) {
+            const Two<A> along_one(-sums[2 * r] * inverse), along_normal(-sums[2 * r + 1] * inverse);
+            Two<A> d[E / 2], normal[E / 2];
+            ring.read(now, r, 0, d);
+            ring.read(now, r, 1, normal);
 #pragma unroll
-                for (int q = 0; q < E / 2; ++q) d[q] = d[q] + normal[q];
+            for (int q = 0; q < E / 2; ++q)
+                d[q] = rstd[r] * fma((normal[q] + away[r]) * rstd[r], along_normal, fma(d[q], weight[q], along_one));
+            const bool live = turn < place.there[r];
+            if (RESIDUAL) {
+                if (added) {
+                    ring.read(now, r, ARRAYS - 1, normal);
+#pragma unroll
+                    for (int q = 0; q < E / 2; ++q) d[q] = d[q] + normal[q];
+                }
+                if (p.dresidual.data != nullptr && live) place.store(dresidual + r * p.dresidual.stride, d, whole);
+                if (p.draw.threshold != 0) drop<V>(draws, (unsigned long long)(row + r) * p.cols + place.at, place.hop(), scale, d);
             }
-            if (p.dresidual.data != nullptr && live)
-#pragma unroll
-                for (int k = 0; k < K; ++k) place.store(dresidual, k, narrow_pack<T, V>(d, k), whole);
-            if (p.draw.threshold != 0)
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-                    drop<V>(draws, (unsigned long long)row * p.cols + place.at + k * place.hop, scale, d, k);
+            if (live) place.store(dx + r * p.dx.stride, d, whole);
         }
-        if (live)
-#pragma unroll
-            for (int k = 0; k < K; ++k) place.store(dx, k, narrow_pack<T, V>(d, k), whole);
+        free = now;
+        now = now == ring.stage(STAGES - 1) ? ring.stage(0) : now + Ring::STAGE_BYTES;
         row += place.step;
         dx += p.dx.advance;
-        dresidual += p.dresidual.advance;
-        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        if (RESIDUAL) dresidual += p.dresidual.advance;
     }
 
     if (p.dweight == nullptr && p.dbias == nullptr) return;
@@ -520,25 +646,26 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
     A* const partial = static_cast<A*>(p.partial) + (long long)(blockIdx.x / shape.cluster) * 2 * p.cols;
     // Groups within a warp by shuffles, those of different warps (or warp groups) through shared memory, [team][2][width].
     const int threads = shape.threads_per_row, width = threads * E;
-    for (int offset = 16; offset >= threads; offset /= 2)
+    if (SPAN != 32)
+        for (int offset = 16; offset >= threads; offset /= 2)
 #pragma unroll
-        for (int q = 0; q < E / 2; ++q) {
-            dweight[q].v.x += __shfl_xor_sync(0xffffffffu, dweight[q].v.x, offset);
-            dweight[q].v.y += __shfl_xor_sync(0xffffffffu, dweight[q].v.y, offset);
-            dbias[q].v.x += __shfl_xor_sync(0xffffffffu, dbias[q].v.x, offset);
-            dbias[q].v.y += __shfl_xor_sync(0xffffffffu, dbias[q].v.y, offset);
-        }
-    const int teams = threads < 32 ? (int)blockDim.x / 32 : shape.groups;
-    const int team = threads < 32 ? (int)threadIdx.x / 32 : place.group;
+            for (int q = 0; q < E / 2; ++q) {
+                const auto w = dweight[q].both(), b = dbias[q].both();
+                dweight[q] = dweight[q] + Two<A>(__shfl_xor_sync(0xffffffffu, w.x, offset), __shfl_xor_sync(0xffffffffu, w.y, offset));
+                dbias[q] = dbias[q] + Two<A>(__shfl_xor_sync(0xffffffffu, b.x, offset), __shfl_xor_sync(0xffffffffu, b.y, offset));
+            }
+    const int teams = SPAN != 32 ? (int)blockDim.x / 32 : shape.groups;
+    const int team = SPAN != 32 ? (int)threadIdx.x / 32 : place.group;
     A* const tile = reinterpret_cast<A*>(dynamic);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();  // the ring is no longer read or written
-    if (threads >= 32 || (int)(threadIdx.x % 32) < threads)
+    if (SPAN == 32 || (int)(threadIdx.x % 32) < threads)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int c = (e / V) * place.hop + place.t * V + e % V;
-            tile[team * 2 * width + c] = e % 2 == 0 ? dweight[e / 2].v.x : dweight[e / 2].v.y;
-            tile[team * 2 * width + width + c] = e % 2 == 0 ? dbias[e / 2].v.x : dbias[e / 2].v.y;
+            const int c = place.at - place.begin + e / V * place.hop() + e % V;
+            const auto w = dweight[e / 2].both(), b = dbias[e / 2].both();
+            tile[team * 2 * width + c] = e % 2 == 0 ? w.x : w.y;
+            tile[team * 2 * width + width + c] = e % 2 == 0 ? b.x : b.y;
         }
     __syncthreads();
     for (int c = threadIdx.x; c < place.end - place.begin; c += blockDim.x) {
@@ -589,14 +716,14 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
         T* y = static_cast<T*>(p.y.data) + row * p.y.stride;
         for (long long c = ((long long)blockIdx.x * threads_per_row + t) * V; c < p.cols; c += (long long)gridDim.x * threads_per_row * V) {
             const int end = p.cols - c < V ? (int)(p.cols - c) : V;
-            Pack<T, V> v = load_pack<T, V>(x + c, 0, end);
+            Pack<T, V> v = load_pack<T, V>(x + c, end);
             if (p.draw.threshold != 0) {
                 bool keep[V];
                 draws.keep((unsigned long long)row * p.cols + c, keep);
 #pragma unroll
                 for (int i = 0; i < V; ++i) v.v[i] = narrow<T>(keep[i] ? widen(v.v[i]) * scale : (A)0);
             }
-            store_pack<T, V>(y + c, 0, end, v);
+            store_pack<T, V>(y + c, end, v);
         }
     }
 }
@@ -624,49 +751,55 @@ cudaError_t launch_rows(void (*kernel)(P...), unsigned grid, unsigned threads, s
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-template <typename T>
-cudaError_t norm_forward_launch(const NormForwardArgs& given, cudaStream_t stream) {
-    NormForwardArgs a = given;
-    constexpr int V = 16 / sizeof(T);
+template <typename T, int V, bool RESIDUAL>
+cudaError_t launch_forward(NormForwardArgs a, cudaStream_t stream) {
     const RowShape s = row_shape(a.cols, norm_elements(sizeof(T)));
-    const int threads = s.threads_per_row * s.groups;
-    const long long batches = (a.rows + s.groups - 1) / s.groups;
-    const long long resident = NORM_SMS * std::max(1, NORM_MAX_THREADS / threads) / s.cluster;
-    const unsigned grid = (unsigned)((batches < resident ? batches : resident) * s.cluster);
-    for (RowArray* r : {&a.x, &a.residual, &a.h, &a.y}) r->advance = (long long)(grid / s.cluster) * s.groups * r->stride;
-    const bool wide = rows_aligned(a.x, a.rows, sizeof(T)) && rows_aligned(a.residual, a.rows, sizeof(T)) &&
-                      rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.y, a.rows, sizeof(T));
-    const bool residual = a.residual.data != nullptr || a.h.data != nullptr || a.draw.threshold != 0;
-    auto kernel = wide ? (residual ? norm_forward_kernel<T, V, true> : norm_forward_kernel<T, V, false>)
-                       : (residual ? norm_forward_kernel<T, 1, true> : norm_forward_kernel<T, 1, false>);
-    const size_t ring = norm_ring_bytes(sizeof(T), residual ? 2 : 1);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring * NORM_MAX_THREADS));
-    return e != cudaSuccess ? e : launch_rows(kernel, grid, threads, ring * threads, s.cluster, stream, a, s);
+    const int threads = s.threads_per_row * s.groups, together = s.groups * norm_forward_rows(sizeof(T), V > 1);
+    const long long batches = (a.rows + together - 1) / together, resident = NORM_SMS * (NORM_MAX_THREADS / threads) / s.cluster;
+    const long long clusters = std::min(batches, resident);
+    for (RowArray* r : {&a.x, &a.residual, &a.h, &a.y}) r->advance = clusters * together * r->stride;
+    auto kernel = s.threads_per_row >= 32 ? norm_forward_kernel<T, V, 32, RESIDUAL> : norm_forward_kernel<T, V, 0, RESIDUAL>;
+    const size_t each = norm_forward_shared(sizeof(T), V > 1, RESIDUAL);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
+    return e != cudaSuccess ? e : launch_rows(kernel, (unsigned)(clusters * s.cluster), threads, each * threads, s.cluster, stream, a, s);
 }
 
 template <typename T>
-cudaError_t norm_backward_launch(const NormBackwardArgs& given, cudaStream_t stream) {
-    NormBackwardArgs a = given;
-    using A = typename Accumulator<T>::type;
+cudaError_t norm_forward_launch(const NormForwardArgs& a, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
+    const bool wide = rows_aligned(a.x, a.rows, sizeof(T)) && rows_aligned(a.residual, a.rows, sizeof(T)) &&
+                      rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.y, a.rows, sizeof(T));
+    if (a.residual.data != nullptr || a.h.data != nullptr || a.draw.threshold != 0)
+        return wide ? launch_forward<T, V, true>(a, stream) : launch_forward<T, 1, true>(a, stream);
+    return wide ? launch_forward<T, V, false>(a, stream) : launch_forward<T, 1, false>(a, stream);
+}
+
+template <typename T, int V, bool RESIDUAL>
+cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
+    using A = typename Accumulator<T>::type;
     const RowShape s = row_shape(a.cols, norm_elements(sizeof(T)));
-    const int threads = s.threads_per_row * s.groups;
-    const int partials = norm_partials(a.rows, s);
-    const unsigned grid = (unsigned)partials * s.cluster;
-    for (RowArray* r : {&a.dy, &a.dh, &a.h, &a.dx, &a.dresidual}) r->advance = (long long)partials * s.groups * r->stride;
-    const bool wide = rows_aligned(a.dy, a.rows, sizeof(T)) && rows_aligned(a.dh, a.rows, sizeof(T)) &&
-                      rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.dx, a.rows, sizeof(T)) &&
-                      rows_aligned(a.dresidual, a.rows, sizeof(T));
-    const bool residual = a.dh.data != nullptr || a.dresidual.data != nullptr || a.draw.threshold != 0;
-    auto kernel = wide ? (residual ? norm_backward_kernel<T, V, true> : norm_backward_kernel<T, V, false>)
-                       : (residual ? norm_backward_kernel<T, 1, true> : norm_backward_kernel<T, 1, false>);
+    const int threads = s.threads_per_row * s.groups, rows_at_once = norm_backward_rows(sizeof(T), V > 1);
+    const int partials = norm_partials(a.rows, rows_at_once, s);
+    for (RowArray* r : {&a.dy, &a.dh, &a.h, &a.dx, &a.dresidual}) r->advance = (long long)partials * s.groups * rows_at_once * r->stride;
+    auto kernel = s.threads_per_row >= 32 ? norm_backward_kernel<T, V, 32, RESIDUAL> : norm_backward_kernel<T, V, 0, RESIDUAL>;
     // The ring's space later holds the groups' shares of the parameters' gradients: two values for each element.
-    const size_t each = std::max(norm_ring_bytes(sizeof(T), residual ? 3 : 2), 2 * norm_elements(sizeof(T)) * sizeof(A));
+    const size_t each = std::max(norm_backward_shared(sizeof(T), V > 1, RESIDUAL), 2 * norm_elements(sizeof(T)) * sizeof(A));
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
-    if (e == cudaSuccess) e = launch_rows(kernel, grid, threads, each * threads, s.cluster, stream, a, s);
+    if (e == cudaSuccess) e = launch_rows(kernel, (unsigned)(partials * s.cluster), threads, each * threads, s.cluster, stream, a, s);
     if (e != cudaSuccess || partials == 1 || (a.dweight == nullptr && a.dbias == nullptr)) return e;
     norm_join_kernel<T><<<dim3((a.cols + 31) / 32, 2), 256, 0, stream>>>(a, partials);
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t norm_backward_launch(const NormBackwardArgs& a, cudaStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = rows_aligned(a.dy, a.rows, sizeof(T)) && rows_aligned(a.dh, a.rows, sizeof(T)) &&
+                      rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.dx, a.rows, sizeof(T)) &&
+                      rows_aligned(a.dresidual, a.rows, sizeof(T));
+    if (a.dh.data != nullptr || a.dresidual.data != nullptr || a.draw.threshold != 0)
+        return wide ? launch_backward<T, V, true>(a, stream) : launch_backward<T, 1, true>(a, stream);
+    return wide ? launch_backward<T, V, false>(a, stream) : launch_backward<T, 1, false>(a, stream);
 }
 
 template <typename T>
