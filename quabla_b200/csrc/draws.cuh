@@ -32,36 +32,28 @@ struct DrawStream {
         threshold = d.threshold;
     }
     static constexpr unsigned long long GAMMA = 0x9e3779b97f4a7c15ull;
+    // The generator's output function up to its last step, z ^ (z >> 31).
     static __device__ __forceinline__ unsigned long long mix(unsigned long long z) {
         z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
-        z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
-        return z ^ (z >> 31);
+        return (z ^ (z >> 27)) * 0x94d049bb133111ebull;
     }
-    // Keep decisions of the V consecutive elements from `index` (row-major, from 0) on.
-    template <int V> __device__ __forceinline__ void keep(unsigned long long index, bool (&kept)[V]) const {
-        const unsigned long long e = index + odd;
-        unsigned long long at = state + ((e >> 1) + 1) * GAMMA;  // of the word that holds e
-        if constexpr (V == 1) {
-            const unsigned long long z = mix(at);
-            kept[0] = ((e & 1) ? (unsigned int)(z >> 32) : (unsigned int)z) >= threshold;
-        } else if ((e & 1) == 0) {
-#pragma unroll
-            for (int j = 0; j < V; j += 2) {
-                const unsigned long long z = mix(at);
-                at += GAMMA;
-                kept[j] = (unsigned int)z >= threshold;
-                kept[j + 1] = (unsigned int)(z >> 32) >= threshold;
-            }
-        } else {
-            unsigned long long z = mix(at);
-#pragma unroll
-            for (int j = 0; j < V; j += 2) {
-                kept[j] = (unsigned int)(z >> 32) >= threshold;
-                at += GAMMA;
-                z = mix(at);
-                kept[j + 1] = (unsigned int)z >= threshold;
-            }
-        }
+    __device__ __forceinline__ bool low_kept(unsigned long long z) const { return (unsigned int)(z ^ (z >> 31)) >= threshold; }
+    // The last step changes no more of the high half than its lowest bit, and that only where its highest is set.  A
+    // threshold up to 2^31 cannot tell, nor can an even one; for an odd one above, FLIP (the integer units are what
+    // bounds 16-bit dropout: without it two of their eleven instructions for an element's half of a word go).
+    template <bool FLIP> __device__ __forceinline__ bool high_kept(unsigned long long z) const {
+        return ((unsigned int)(z >> 32) ^ (FLIP ? 1u : 0u)) >= threshold;
+    }
+    __device__ __forceinline__ bool flips() const { return threshold > 0x80000000u && (threshold & 1u) != 0; }
+    // Element `index` (row-major, from 0; elements before the first have some bits or other) is the low half of the word
+    // at `at(index)` if half(index) is 0, its high half otherwise; the next word is GAMMA further on.
+    __device__ __forceinline__ unsigned long long at(long long index) const {
+        return state + (unsigned long long)(((index + odd) >> 1) + 1) * GAMMA;
+    }
+    __device__ __forceinline__ unsigned int half(long long index) const { return ((unsigned int)index + odd) & 1u; }
+    __device__ __forceinline__ bool kept(long long index) const {
+        const unsigned long long z = mix(at(index)), bits = z ^ (z >> 31);
+        return (half(index) ? (unsigned int)(bits >> 32) : (unsigned int)bits) >= threshold;
     }
 };
 

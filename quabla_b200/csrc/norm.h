@@ -55,20 +55,15 @@ __host__ __device__ constexpr int norm_elements(size_t element_bytes) { return e
 // rows share a turn's reductions, barrier and addresses.
 __host__ __device__ constexpr int norm_forward_rows(size_t element_bytes, bool wide) { return element_bytes == 2 && wide ? 2 : 1; }
 __host__ __device__ constexpr int norm_backward_rows(size_t element_bytes, bool wide) { return element_bytes == 2 && wide ? 2 : 1; }
-// Whether the forward kernel's parameters are in shared memory instead of registers.
-__host__ __device__ constexpr bool norm_forward_shared_columns(size_t element_bytes, bool wide, bool residual) {
-    return element_bytes == 2 && wide && !residual;
-}
 // Turns whose rows are on their way or in work in a thread's slots.
 __host__ __device__ constexpr int norm_forward_stages(size_t element_bytes, bool wide, bool residual) {
-    return norm_forward_shared_columns(element_bytes, wide, residual) ? 2 : residual ? 3 : 4;
+    return residual || norm_forward_rows(element_bytes, wide) == 2 ? 3 : 4;
 }
 __host__ __device__ constexpr int norm_backward_stages(bool residual) { return residual ? 2 : 3; }
-// Shared memory of a thread: its slots, and its columns of weight and bias where they are there.
+// Bytes of a thread's slots.
 constexpr size_t norm_forward_shared(size_t element_bytes, bool wide, bool residual) {
-    const size_t row = norm_elements(element_bytes) * element_bytes;
-    return norm_forward_stages(element_bytes, wide, residual) * norm_forward_rows(element_bytes, wide) * (residual ? 2 : 1) * row +
-           (norm_forward_shared_columns(element_bytes, wide, residual) ? 2 * norm_elements(element_bytes) * 4 : 0);
+    return norm_forward_stages(element_bytes, wide, residual) * norm_forward_rows(element_bytes, wide) * (residual ? 2 : 1) *
+           norm_elements(element_bytes) * element_bytes;
 }
 constexpr size_t norm_backward_shared(size_t element_bytes, bool wide, bool residual) {
     return norm_backward_stages(residual) * norm_backward_rows(element_bytes, wide) * (residual ? 3 : 2) * norm_elements(element_bytes) * element_bytes;

@@ -314,60 +314,65 @@ template <typename T, int V, int ARRAYS, int ROWS, int STAGES> struct RowRing {
     static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory"); }
 };
 
-// A thread's columns of a parameter, 1 or 0 where there is none: in registers, or in slots of its own in shared memory
-// where registers are worth more.
-template <typename T, int V, bool SHARED> struct Columns {
-    using A = typename Accumulator<T>::type;
-    static constexpr int E = norm_elements(sizeof(T)), H = E / 2, W = 16 / sizeof(Two<A>);
-    struct alignas(16) Slot { Two<A> v[W]; };
-    static constexpr int THREAD_BYTES = SHARED ? E * sizeof(A) : 0;
-    Two<A> pairs[SHARED ? 1 : H];
-    Slot* slots;  // [warps][H / W][32]
-    template <typename P>
-    __device__ __forceinline__ Columns(const P& place, const void* params, bool f32, A absent, char* shared) {
-        slots = reinterpret_cast<Slot*>(shared) + threadIdx.x / 32 * (H / W * 32) + threadIdx.x % 32;
+// A thread's columns of a parameter, 1 or 0 where there is none.
+template <typename T, int V, typename P, typename A, int H>
+__device__ __forceinline__ void load_columns(const P& place, const void* params, bool f32, A absent, Two<A> (&pairs)[H]) {
 #pragma unroll
-        for (int q = 0; q < H; ++q) {
-            A v[2];
+    for (int q = 0; q < H; ++q) {
+        A v[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int c = place.at + (2 * q + i) / V * place.hop() + (2 * q + i) % V;
-                v[i] = params != nullptr && c < place.end ? load_param<T, A>(params, f32, c) : absent;
-            }
-            if constexpr (SHARED) slots[q / W * 32].v[q % W] = Two<A>(v[0], v[1]);
-            else pairs[q] = Two<A>(v[0], v[1]);
+        for (int i = 0; i < 2; ++i) {
+            const int c = place.at + (2 * q + i) / V * place.hop() + (2 * q + i) % V;
+            v[i] = params != nullptr && c < place.end ? load_param<T, A>(params, f32, c) : absent;
         }
+        pairs[q] = Two<A>(v[0], v[1]);
     }
-    __device__ __forceinline__ void get(Two<A> (&out)[H]) const {
-        if constexpr (SHARED) {
-#pragma unroll
-            for (int w = 0; w < H / W; ++w) {
-                const Slot slot = slots[w * 32];
-#pragma unroll
-                for (int i = 0; i < W; ++i) out[w * W + i] = slot.v[i];
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < H; ++q) out[q] = pairs[q];
-        }
-    }
-};
+}
 
-// Dropout of a thread's packs of a row; `index` is the row-major number of its first column.
-template <int V, typename A, int H>
-__device__ __forceinline__ void drop(const DrawStream& draws, unsigned long long index, int hop, A scale, Two<A> (&pairs)[H]) {
-    constexpr int K = 2 * H / V;
+// Dropout of PACKS packs of V elements, `hop` columns from one to the next; `index` is the row-major number of the first.
+// Both halves of a word are used; where the elements start with a high half, a pack takes one word more.  (The branches on
+// that hold the whole work: decisions that leave them would have to pass through registers.)
+template <int V, int PACKS, bool FLIP, typename A>
+__device__ __forceinline__ void drop_pairs(const DrawStream& draws, long long index, int hop, A scale, Two<A>* pairs) {
+    const Two<A> factor(scale);
+    const unsigned long long first = draws.at(index);
+    if (draws.half(index) == 0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        bool keep[V];
-        draws.keep(index + k * hop, keep);
+        for (int k = 0; k < PACKS; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            Two<A>& pair = pairs[(k * V + i) / 2];
-            const auto f = pair.both();
-            if (V == 1) pair = k % 2 == 0 ? Two<A>(keep[0] ? f.x * scale : (A)0, f.y) : Two<A>(f.x, keep[0] ? f.y * scale : (A)0);
-            else if (i % 2 == 0) pair = Two<A>(keep[i] ? f.x * scale : (A)0, keep[(i + 1) % V] ? f.y * scale : (A)0);
+            for (int j = 0; j < V / 2; ++j) {
+                const unsigned long long z = DrawStream::mix(first + ((unsigned long long)(k * hop / 2) + j) * DrawStream::GAMMA);
+                const auto f = (pairs[k * V / 2 + j] * factor).both();
+                pairs[k * V / 2 + j] = Two<A>(draws.low_kept(z) ? f.x : (A)0, draws.high_kept<FLIP>(z) ? f.y : (A)0);
+            }
+    } else {
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            const unsigned long long at = first + (unsigned long long)(k * hop / 2) * DrawStream::GAMMA;
+            unsigned long long last = DrawStream::mix(at);
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {
+                const unsigned long long z = DrawStream::mix(at + (j + 1) * DrawStream::GAMMA);
+                const auto f = (pairs[k * V / 2 + j] * factor).both();
+                pairs[k * V / 2 + j] = Two<A>(draws.high_kept<FLIP>(last) ? f.x : (A)0, draws.low_kept(z) ? f.y : (A)0);
+                last = z;
+            }
         }
+    }
+}
+
+template <int V, int PACKS, typename A>
+__device__ __forceinline__ void drop(const DrawStream& draws, long long index, int hop, A scale, Two<A>* pairs) {
+    if constexpr (V == 1) {
+#pragma unroll
+        for (int k = 0; k < PACKS; k += 2) {
+            const auto f = (pairs[k / 2] * Two<A>(scale)).both();
+            pairs[k / 2] = Two<A>(draws.kept(index + k * hop) ? f.x : (A)0, draws.kept(index + (k + 1) * hop) ? f.y : (A)0);
+        }
+    } else if (draws.flips()) {
+        drop_pairs<V, PACKS, true>(draws, index, hop, scale, pairs);
+    } else {
+        drop_pairs<V, PACKS, false>(draws, index, hop, scale, pairs);
     }
 }
 
@@ -377,7 +382,6 @@ __global__ void __maxnreg__(128)
 norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
     constexpr int ARRAYS = RESIDUAL ? 2 : 1, R = norm_forward_rows(sizeof(T), V > 1), STAGES = norm_forward_stages(sizeof(T), V > 1, RESIDUAL);
-    constexpr bool SHARED = norm_forward_shared_columns(sizeof(T), V > 1, RESIDUAL);
     using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
     __shared__ typename RowSum<A, R, SPAN>::Shared shared;
@@ -421,10 +425,9 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
 
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale, inverse = (A)1 / (A)p.cols;
-    using Cols = Columns<T, V, SHARED>;
-    char* const behind = dynamic + Ring::THREAD_BYTES * blockDim.x;
-    const Cols weights(place, p.weight, p.params_f32, (A)1, behind);
-    const Cols biases(place, p.bias, p.params_f32, (A)0, behind + Cols::THREAD_BYTES * blockDim.x);
+    Two<A> weight[E / 2], bias[E / 2];
+    load_columns<T, V>(place, p.weight, p.params_f32, (A)1, weight);
+    load_columns<T, V>(place, p.bias, p.params_f32, (A)0, bias);
 
     const int turns = place.turns(p.rows);
     char *now = ring.stage(0), *free = ring.stage(STAGES - 1);  // the slots in work; those read in the last turn
@@ -437,7 +440,7 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
         for (int r = 0; r < R; ++r) {
             ring.read(now, r, 0, h[r]);
             if (RESIDUAL) {
-                if (p.draw.threshold != 0) drop<V>(draws, (unsigned long long)(row + r) * p.cols + place.at, place.hop(), scale, h[r]);
+                if (p.draw.threshold != 0) drop<V, K>(draws, (row + r) * p.cols + place.at, place.hop(), scale, h[r]);
                 if (added) {
                     Two<A> more[E / 2];
                     ring.read(now, r, ARRAYS - 1, more);
@@ -477,9 +480,6 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
             }
         }
         row_sum(squares);
-        Two<A> weight[E / 2], bias[E / 2];
-        weights.get(weight);
-        biases.get(bias);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const A rstd = reciprocal_root(squares[r] * inverse + (A)p.epsilon);
@@ -562,9 +562,8 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
 
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale, inverse = (A)1 / (A)p.cols;
-    const Columns<T, V, false> weights(place, p.weight, p.params_f32, (A)1, dynamic);
-    const auto& weight = weights.pairs;
-    Two<A> dweight[E / 2], dbias[E / 2];
+    Two<A> weight[E / 2], dweight[E / 2], dbias[E / 2];
+    load_columns<T, V>(place, p.weight, p.params_f32, (A)1, weight);
 #pragma unroll
     for (int q = 0; q < E / 2; ++q) dweight[q] = dbias[q] = Two<A>((A)0);
 
@@ -630,7 +629,7 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
                     for (int q = 0; q < E / 2; ++q) d[q] = d[q] + normal[q];
                 }
                 if (p.dresidual.data != nullptr && live) place.store(dresidual + r * p.dresidual.stride, d, whole);
-                if (p.draw.threshold != 0) drop<V>(draws, (unsigned long long)(row + r) * p.cols + place.at, place.hop(), scale, d);
+                if (p.draw.threshold != 0) drop<V, K>(draws, (row + r) * p.cols + place.at, place.hop(), scale, d);
             }
             if (live) place.store(dx + r * p.dx.stride, d, whole);
         }
@@ -641,6 +640,7 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
         if (RESIDUAL) dresidual += p.dresidual.advance;
     }
 
+    asm volatile("griddepcontrol.launch_dependents;");  // the joining kernel's CTAs may take the places of those that end
     if (p.dweight == nullptr && p.dbias == nullptr) return;
     const bool final = gridDim.x == (unsigned)shape.cluster;  // no other CTA has these columns
     A* const partial = static_cast<A*>(p.partial) + (long long)(blockIdx.x / shape.cluster) * 2 * p.cols;
@@ -695,8 +695,11 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const __grid_constant__ 
     if (out == nullptr) return;
     const A* partial = static_cast<const A*>(p.partial) + (long long)blockIdx.y * p.cols;
     double sum = 0.0;
-    if (c < p.cols)
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial rows are there
+    if (c < p.cols) {
+#pragma unroll 8
         for (int r = lane; r < partials; r += 8) sum += (double)partial[(long long)r * 2 * p.cols + c];
+    }
     sums[lane][threadIdx.x % 32] = sum;
     __syncthreads();
     if (lane != 0 || c >= p.cols) return;
@@ -705,25 +708,86 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const __grid_constant__ 
     store_gradient<T>(out, p.params_f32, c, (A)sum);
 }
 
+// Elements [low, high) of a pack, the others as zeros.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutArgs p, int threads_per_row) {
+__device__ __forceinline__ Pack<T, V> load_part(const T* from, int low, int high) {
+    Pack<T, V> p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.v[i] = i >= low && i < high ? from[i] : narrow<T>((typename Accumulator<T>::type)0);
+    return p;
+}
+
+template <typename T, int V, int PACKS, typename A>
+__device__ __forceinline__ void drop_packs(const DrawStream& draws, long long index, int hop, A scale, Pack<T, V> (&v)[PACKS]) {
+    if (draws.threshold == 0) return;
+    if constexpr (V == 1) {
+#pragma unroll
+        for (int d = 0; d < PACKS; ++d) v[d].v[0] = narrow<T>(draws.kept(index + d * hop) ? widen(v[d].v[0]) * scale : (A)0);
+    } else {
+        Two<A> pairs[PACKS * V / 2];
+        widen_packs<T, V>(v, pairs);
+        drop<V, PACKS>(draws, index, hop, scale, pairs);
+#pragma unroll
+        for (int d = 0; d < PACKS; ++d) v[d] = narrow_pack<T, V>(pairs, d);
+    }
+}
+
+// Dropout alone.  Rows are taken in 16-byte packs from 16-byte boundary to boundary wherever they start, as long as x and y
+// start at the same distance from one (V > 1): pack i of a row holds columns [i * V - shift, (i + 1) * V - shift).  One
+// long row (what a contiguous array is) and many rows are two kernels: in the one row the four packs that a thread has on
+// their way are a constant distance apart in the stream of words; of many rows a thread has two.
+__host__ __device__ constexpr int dropout_depth(bool one_row) { return one_row ? 4 : 2; }
+template <typename T, int V, bool ONE_ROW>
+__global__ void __launch_bounds__(256, ONE_ROW ? 4 : 6) dropout_kernel(const __grid_constant__ DropoutArgs p, long long packs, long long packs_per_row) {
     using A = typename Accumulator<T>::type;
-    const int t = threadIdx.x % threads_per_row, group = threadIdx.x / threads_per_row, groups = blockDim.x / threads_per_row;
+    constexpr int DEPTH = dropout_depth(ONE_ROW);
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale;
-    for (long long row = (long long)blockIdx.y * groups + group; row < p.rows; row += (long long)gridDim.y * groups) {
-        const T* x = static_cast<const T*>(p.x.data) + row * p.x.stride;
-        T* y = static_cast<T*>(p.y.data) + row * p.y.stride;
-        for (long long c = ((long long)blockIdx.x * threads_per_row + t) * V; c < p.cols; c += (long long)gridDim.x * threads_per_row * V) {
-            const int end = p.cols - c < V ? (int)(p.cols - c) : V;
-            Pack<T, V> v = load_pack<T, V>(x + c, end);
-            if (p.draw.threshold != 0) {
-                bool keep[V];
-                draws.keep((unsigned long long)row * p.cols + c, keep);
+    const int hop = (int)(gridDim.x * blockDim.x);
+    auto shift_of = [](const T* x) { return V == 1 ? 0 : (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % V); };
+    for (long long first = (long long)blockIdx.x * blockDim.x + threadIdx.x; first < packs; first += (long long)DEPTH * hop) {
+        if constexpr (ONE_ROW) {
+            const T* const x = static_cast<const T*>(p.x.data);
+            T* const y = static_cast<T*>(p.y.data);
+            const long long c = first * V - shift_of(x);
+            if (c >= 0 && c + (long long)(DEPTH - 1) * hop * V + V <= p.cols) {
+                Pack<T, V> v[DEPTH];
 #pragma unroll
-                for (int i = 0; i < V; ++i) v.v[i] = narrow<T>(keep[i] ? widen(v.v[i]) * scale : (A)0);
+                for (int d = 0; d < DEPTH; ++d) v[d] = *reinterpret_cast<const Pack<T, V>*>(x + c + d * hop * V);
+                drop_packs(draws, c, hop * V, scale, v);
+#pragma unroll
+                for (int d = 0; d < DEPTH; ++d) *reinterpret_cast<Pack<T, V>*>(y + c + d * hop * V) = v[d];
+                continue;
             }
-            store_pack<T, V>(y + c, end, v);
+        }
+        Pack<T, V> v[DEPTH];
+        long long row[DEPTH], c[DEPTH];
+        int low[DEPTH], high[DEPTH];
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const long long pack = first + (long long)d * hop;
+            row[d] = ONE_ROW ? 0 : packs <= 0xffffffffll ? (long long)((unsigned int)pack / (unsigned int)packs_per_row) : pack / packs_per_row;
+            const T* x = static_cast<const T*>(p.x.data) + row[d] * p.x.stride;
+            c[d] = (pack - row[d] * packs_per_row) * V - shift_of(x);
+            const long long left = p.cols - c[d];
+            low[d] = c[d] < 0 ? (int)-c[d] : 0;
+            high[d] = pack >= packs || left <= 0 ? 0 : left < V ? (int)left : V;
+            if (low[d] == 0 && high[d] == V) v[d] = *reinterpret_cast<const Pack<T, V>*>(x + c[d]);
+            else v[d] = load_part<T, V>(x + c[d], low[d], high[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (high[d] == 0) continue;
+            Pack<T, V> one[1] = {v[d]};
+            drop_packs(draws, row[d] * p.cols + c[d], 0, scale, one);
+            T* y = static_cast<T*>(p.y.data) + row[d] * p.y.stride + c[d];
+            if (low[d] == 0 && high[d] == V) {
+                *reinterpret_cast<Pack<T, V>*>(y) = one[0];
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (i >= low[d] && i < high[d]) y[i] = one[0].v[i];
+            }
         }
     }
 }
@@ -787,8 +851,16 @@ cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
     if (e == cudaSuccess) e = launch_rows(kernel, (unsigned)(partials * s.cluster), threads, each * threads, s.cluster, stream, a, s);
     if (e != cudaSuccess || partials == 1 || (a.dweight == nullptr && a.dbias == nullptr)) return e;
-    norm_join_kernel<T><<<dim3((a.cols + 31) / 32, 2), 256, 0, stream>>>(a, partials);
-    return cudaGetLastError();
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((a.cols + 31) / 32, 2);
+    config.blockDim = dim3(256);
+    config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, norm_join_kernel<T>, a, partials);
 }
 
 template <typename T>
@@ -810,18 +882,18 @@ cudaError_t dropout_launch(const DropoutArgs& given, cudaStream_t stream) {
         a.cols *= a.rows;
         a.rows = 1;
     }
-    const bool wide = rows_aligned(a.x, a.rows, sizeof(T)) && rows_aligned(a.y, a.rows, sizeof(T));
-    const long long packs = wide ? (a.cols + V - 1) / V : a.cols;
-    int threads_per_row = 1;
-    while (threads_per_row < packs && threads_per_row < 256) threads_per_row *= 2;
-    const int groups = 256 / threads_per_row;
-    const long long resident = NORM_SMS * 8;
-    const long long across = (packs + threads_per_row - 1) / threads_per_row, down = (a.rows + groups - 1) / groups;
-    const long long gx = across < resident ? across : resident;
-    const long long most = (resident + gx - 1) / gx, gy = down < most ? down : most;
-    const dim3 grid((unsigned)gx, (unsigned)gy);
-    if (wide) dropout_kernel<T, V><<<grid, 256, 0, stream>>>(a, threads_per_row);
-    else dropout_kernel<T, 1><<<grid, 256, 0, stream>>>(a, threads_per_row);
+    const bool wide = (reinterpret_cast<uintptr_t>(a.x.data) - reinterpret_cast<uintptr_t>(a.y.data)) % 16 == 0 &&
+                      (a.rows <= 1 || (a.x.stride - a.y.stride) * (long long)sizeof(T) % 16 == 0);
+    const long long per_row = wide ? (a.cols + V - 1) / V + 1 : a.cols;  // one more where a row starts between boundaries
+    const long long packs = per_row * a.rows, each = 256 * dropout_depth(a.rows == 1);
+    // Small arrays: a pack for each thread and as many CTAs as that takes.  Large ones: 16-bit rows are bound by the integer
+    // units and 8 CTAs for each SM do best (16384 x 8192 bfloat16 108 us, with 24 119), others by memory and 24 (8192 x 8192
+    // float32 86 us, with 8 95).
+    const long long spread = (packs + 255) / 256, deep = (packs + each - 1) / each;
+    const unsigned grid = (unsigned)(spread <= NORM_SMS * 4 ? spread : std::max<long long>(NORM_SMS * 4, std::min<long long>(deep, NORM_SMS * (sizeof(T) == 2 && a.rows == 1 ? 8 : 24))));
+    auto kernel = a.rows == 1 ? (wide ? dropout_kernel<T, V, true> : dropout_kernel<T, 1, true>)
+                              : (wide ? dropout_kernel<T, V, false> : dropout_kernel<T, 1, false>);
+    kernel<<<grid, 256, 0, stream>>>(a, packs, per_row);
     return cudaGetLastError();
 }
 

@@ -129,6 +129,47 @@ def test_dropout(cuda_device, dtype, rows, cols, pad, shift, counter):
     assert y.outside_untouched()
 
 
+def _key_of_word(word):
+    """The key whose first word is `word`: the generator's output function backwards."""
+    mask = (1 << 64) - 1
+
+    def unshift(z, by):
+        out = z
+        for _ in range(64 // by + 1):
+            out = z ^ (out >> by)
+        return out
+
+    z = unshift(word, 31)
+    z = unshift((z * pow(0x94D049BB133111EB, -1, 1 << 64)) & mask, 27)
+    z = unshift((z * pow(0xBF58476D1CE4E5B9, -1, 1 << 64)) & mask, 30)
+    return (z - 0x9E3779B97F4A7C15) & mask
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rate", [0.1, 0.5, 0.7, 0.9, 0.25, 1.0 - 2.0**-32, 0.5 + 2.0**-32, 2.0**-32])
+@pytest.mark.parametrize("residual", [False, True])
+def test_elements_at_the_threshold(cuda_device, dtype, rate, residual):
+    # Words whose halves lie at the threshold and next to it, as low and as high halves, in packs that start with either.
+    import torch
+
+    threshold = int(rate * 2**32)
+    halves = [h for h in range(threshold - 2, threshold + 3) if 0 <= h < 2**32]
+    for half in halves:
+        for word in (half, half << 32, half << 32 | 0xFFFFFFFF, half | 0xFFFFFFFF << 32):
+            key = qb.random.Key(_key_of_word(word))
+            assert int(qb.random._stream(key.value, 1)[0]) == word
+            for counter in (0, 1):
+                kept = nu.mask(key, 1, 64, rate, counter)
+                x = nu.Rows(1, 64, dtype, values=torch.ones(1, 64, dtype=torch.float64))
+                y, h = nu.Rows(1, 64, dtype), nu.Rows(1, 64, dtype)
+                if residual:
+                    nu.dropout_layer_norm(dtype, dtype, x, None, rate, key.value, counter, None, None, h, y, None, None)
+                    assert ((h.view != 0) == kept).all()
+                else:
+                    nu.dropout(dtype, x, rate, key.value, counter, y)
+                    assert ((y.view != 0) == kept).all()
+
+
 def test_dropout_at_rate_zero_copies_and_rows_with_different_strides(cuda_device):
     x = nu.Rows(7, 24, "bfloat16", 8, 0, nu.normal(1, 7, 24))
     y = nu.Rows(7, 24, "bfloat16", 1, 0)
