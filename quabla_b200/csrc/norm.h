@@ -54,7 +54,11 @@ __host__ __device__ constexpr int norm_elements(size_t element_bytes) { return e
 // Rows that a group works on at once.  16-bit rows that come 16 bytes at a time are bound by instruction issue: two
 // rows share a turn's reductions, barrier and addresses.
 __host__ __device__ constexpr int norm_forward_rows(size_t element_bytes, bool wide) { return element_bytes == 2 && wide ? 2 : 1; }
-__host__ __device__ constexpr int norm_backward_rows(size_t element_bytes, bool wide) { return element_bytes == 2 && wide ? 2 : 1; }
+// Rows that share a warp have no barrier to share and are worked on one at a time in the backward pass, whose registers
+// two would not fit (262144 x 128 bfloat16 50 us with two).
+__host__ __device__ constexpr int norm_backward_rows(size_t element_bytes, bool wide, bool whole_warps) {
+    return element_bytes == 2 && wide && whole_warps ? 2 : 1;
+}
 // Turns whose rows are on their way or in work in a thread's slots.
 __host__ __device__ constexpr int norm_forward_stages(size_t element_bytes, bool wide, bool residual) {
     return residual || norm_forward_rows(element_bytes, wide) == 2 ? 3 : 4;
@@ -65,8 +69,8 @@ constexpr size_t norm_forward_shared(size_t element_bytes, bool wide, bool resid
     return norm_forward_stages(element_bytes, wide, residual) * norm_forward_rows(element_bytes, wide) * (residual ? 2 : 1) *
            norm_elements(element_bytes) * element_bytes;
 }
-constexpr size_t norm_backward_shared(size_t element_bytes, bool wide, bool residual) {
-    return norm_backward_stages(residual) * norm_backward_rows(element_bytes, wide) * (residual ? 3 : 2) * norm_elements(element_bytes) * element_bytes;
+constexpr size_t norm_backward_shared(size_t element_bytes, bool wide, bool whole_warps, bool residual) {
+    return norm_backward_stages(residual) * norm_backward_rows(element_bytes, wide, whole_warps) * (residual ? 3 : 2) * norm_elements(element_bytes) * element_bytes;
 }
 constexpr int NORM_MAX_THREADS = 512;
 constexpr int NORM_MAX_CLUSTER = 8;

@@ -515,7 +515,7 @@ template <typename T, int V, int SPAN, bool RESIDUAL>
 __global__ void __maxnreg__(128)
 norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
-    constexpr int ARRAYS = RESIDUAL ? 3 : 2, R = norm_backward_rows(sizeof(T), V > 1), STAGES = norm_backward_stages(RESIDUAL);
+    constexpr int ARRAYS = RESIDUAL ? 3 : 2, R = norm_backward_rows(sizeof(T), V > 1, SPAN == 32), STAGES = norm_backward_stages(RESIDUAL);
     using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
     __shared__ typename RowSum<A, 2 * R, SPAN>::Shared shared;
@@ -842,12 +842,12 @@ template <typename T, int V, bool RESIDUAL>
 cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
     using A = typename Accumulator<T>::type;
     const RowShape s = row_shape(a.cols, norm_elements(sizeof(T)));
-    const int threads = s.threads_per_row * s.groups, rows_at_once = norm_backward_rows(sizeof(T), V > 1);
+    const int threads = s.threads_per_row * s.groups, rows_at_once = norm_backward_rows(sizeof(T), V > 1, s.threads_per_row >= 32);
     const int partials = norm_partials(a.rows, rows_at_once, s);
     for (RowArray* r : {&a.dy, &a.dh, &a.h, &a.dx, &a.dresidual}) r->advance = (long long)partials * s.groups * rows_at_once * r->stride;
     auto kernel = s.threads_per_row >= 32 ? norm_backward_kernel<T, V, 32, RESIDUAL> : norm_backward_kernel<T, V, 0, RESIDUAL>;
     // The ring's space later holds the groups' shares of the parameters' gradients: two values for each element.
-    const size_t each = std::max(norm_backward_shared(sizeof(T), V > 1, RESIDUAL), 2 * norm_elements(sizeof(T)) * sizeof(A));
+    const size_t each = std::max(norm_backward_shared(sizeof(T), V > 1, s.threads_per_row >= 32, RESIDUAL), 2 * norm_elements(sizeof(T)) * sizeof(A));
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
     if (e == cudaSuccess) e = launch_rows(kernel, (unsigned)(partials * s.cluster), threads, each * threads, s.cluster, stream, a, s);
     if (e != cudaSuccess || partials == 1 || (a.dweight == nullptr && a.dbias == nullptr)) return e;
