@@ -15,6 +15,7 @@ struct Draw {
     unsigned long long key = 0;
     unsigned long long counter = 0;                  // index of element (0, 0) in the stream of halves
     const unsigned long long* d_counter = nullptr;   // added to counter when the kernel runs
+    bool active = false;                             // rate > 0 (the threshold of a rate below 2^-32 is 0 all the same)
     unsigned int threshold = 0;                      // floor(rate * 2^32); an element is kept iff its half >= threshold
     double scale = 1.0;                              // 1 / (1 - rate)
 };
@@ -25,11 +26,13 @@ struct DrawStream {
     unsigned long long state;
     unsigned int odd;
     unsigned int threshold;
+    bool active;
     __device__ __forceinline__ explicit DrawStream(const Draw& d) {
         const unsigned long long first = d.counter + (d.d_counter != nullptr ? *d.d_counter : 0ull);
         state = d.key + (first >> 1) * 0x9e3779b97f4a7c15ull;
         odd = (unsigned int)first & 1u;
         threshold = d.threshold;
+        active = d.active;
     }
     static constexpr unsigned long long GAMMA = 0x9e3779b97f4a7c15ull;
     // The generator's output function up to its last step, z ^ (z >> 31).

@@ -90,6 +90,7 @@ qb200_status make_draw(const char* op, double rate, uint64_t key, uint64_t count
     out->key = key;
     out->counter = counter;
     out->d_counter = reinterpret_cast<const unsigned long long*>(d_counter);
+    out->active = rate > 0.0;
     out->threshold = (unsigned int)std::floor(rate * 4294967296.0);
     out->scale = 1.0 / (1.0 - rate);
     return QB200_OK;

@@ -339,7 +339,7 @@ enum class Draws { NONE, PLAIN, ANY };
 template <Draws D> using DrawsTag = std::integral_constant<Draws, D>;
 template <int V>
 __device__ __forceinline__ Draws draws_of(const DrawStream& draws, int cols) {
-    if (draws.threshold == 0) return Draws::NONE;
+    if (!draws.active) return Draws::NONE;
     return V > 1 && draws.odd == 0 && cols % 2 == 0 && !draws.flips() ? Draws::PLAIN : Draws::ANY;
 }
 
@@ -766,7 +766,7 @@ __device__ __forceinline__ Pack<T, V> load_part(const T* from, int low, int high
 
 template <typename T, int V, int PACKS, typename A>
 __device__ __forceinline__ void drop_packs(const DrawStream& draws, long long index, int hop, A scale, Pack<T, V> (&v)[PACKS]) {
-    if (draws.threshold == 0) return;
+    if (!draws.active) return;
     if constexpr (V == 1) {
 #pragma unroll
         for (int d = 0; d < PACKS; ++d) v[d].v[0] = narrow<T>(draws.kept(index + d * hop) ? widen(v[d].v[0]) * scale : (A)0);
@@ -880,7 +880,7 @@ cudaError_t norm_forward_launch(const NormForwardArgs& a, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     const bool wide = rows_aligned(a.x, a.rows, sizeof(T)) && rows_aligned(a.residual, a.rows, sizeof(T)) &&
                       rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.y, a.rows, sizeof(T));
-    if (a.residual.data != nullptr || a.h.data != nullptr || a.draw.threshold != 0)
+    if (a.residual.data != nullptr || a.h.data != nullptr || a.draw.active)
         return wide ? launch_forward<T, V, true>(a, stream) : launch_forward<T, 1, true>(a, stream);
     return wide ? launch_forward<T, V, false>(a, stream) : launch_forward<T, 1, false>(a, stream);
 }
@@ -917,7 +917,7 @@ cudaError_t norm_backward_launch(const NormBackwardArgs& a, cudaStream_t stream)
     const bool wide = rows_aligned(a.dy, a.rows, sizeof(T)) && rows_aligned(a.dh, a.rows, sizeof(T)) &&
                       rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.dx, a.rows, sizeof(T)) &&
                       rows_aligned(a.dresidual, a.rows, sizeof(T));
-    if (a.dh.data != nullptr || a.dresidual.data != nullptr || a.draw.threshold != 0)
+    if (a.dh.data != nullptr || a.dresidual.data != nullptr || a.draw.active)
         return wide ? launch_backward<T, V, true>(a, stream) : launch_backward<T, 1, true>(a, stream);
     return wide ? launch_backward<T, V, false>(a, stream) : launch_backward<T, 1, false>(a, stream);
 }
@@ -941,8 +941,7 @@ cudaError_t dropout_launch(const DropoutArgs& given, cudaStream_t stream) {
     const unsigned grid = (unsigned)(spread <= NORM_SMS * 4 ? spread : std::max<long long>(NORM_SMS * 4, std::min<long long>(deep, NORM_SMS * (sizeof(T) == 2 && a.rows == 1 ? 8 : 24))));
     auto kernel = a.rows == 1 ? (wide ? dropout_kernel<T, V, true> : dropout_kernel<T, 1, true>)
                               : (wide ? dropout_kernel<T, V, false> : dropout_kernel<T, 1, false>);
-    kernel<<<grid, 256, 0, stream>>>(a, packs, per_row);
-    return cudaGetLastError();
+    return launch_rows(kernel, grid, 256, 0, 1, stream, a, packs, per_row);
 }
 
 #define QB_INSTANTIATE_NORM(T)                                                              \

@@ -181,6 +181,17 @@ def test_dropout_at_rate_zero_copies_and_rows_with_different_strides(cuda_device
     assert ((z.wide() == 2 * x.wide()) | ~kept).all() and (z.wide()[~kept] == 0).all()
 
 
+@pytest.mark.parametrize("rate", [1e-12, 2.0**-33])
+def test_a_rate_below_the_draws_resolution_scales_and_drops_nothing(cuda_device, rate):
+    x, y, h = nu.Rows(3, 50, "float64", values=nu.normal(1, 3, 50)), nu.Rows(3, 50, "float64"), nu.Rows(3, 50, "float64")
+    want = x.view * (1.0 / (1.0 - rate))
+    assert not (want == x.view).all()
+    nu.dropout("float64", x, rate, 1, 0, y)
+    assert (y.view == want).all()
+    nu.dropout_layer_norm("float64", "float64", x, None, rate, 1, 0, None, None, h, y, None, None)
+    assert (h.view == want).all()
+
+
 def test_dropped_elements_are_zero_whatever_they_hold(cuda_device):
     import torch
 
