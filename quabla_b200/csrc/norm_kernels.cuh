@@ -547,6 +547,25 @@ __device__ __forceinline__ void store_gradient(void* out, bool f32, int c, A v) 
     else static_cast<T*>(out)[c] = narrow<T>(v);
 }
 
+// A thread's sums to its columns; `wide`: 16-byte stores where a pack is whole.
+template <typename A, int V, int K, typename P, int H>
+__device__ __forceinline__ void store_sums(A* at, const P& place, const Two<A> (&pairs)[H], bool wide) {
+    constexpr int W = 16 / sizeof(A);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const Pack<A, V> sums = narrow_pack<A, V>(pairs, k);
+        A* const to = at + k * place.hop();
+        if (V % W == 0 && wide && k < place.solid) {
+#pragma unroll
+            for (int i = 0; i < V; i += W) *reinterpret_cast<Pack<A, W>*>(to + i) = *reinterpret_cast<const Pack<A, W>*>(&sums.v[i]);
+        } else {
+            store_pack<A, 1>(to, place.count(k), Pack<A, 1>{{sums.v[0]}});
+#pragma unroll
+            for (int i = 1; i < V; ++i) store_pack<A, 1>(to + i, place.count(k) - i, Pack<A, 1>{{sums.v[i]}});
+        }
+    }
+}
+
 // RESIDUAL: dh is added to the row's gradient, which goes to dresidual, and through dropout's mask to dx.
 // Threads keep their columns' share of dweight and dbias in registers over all rows of the CTA; at the end the CTA's
 // groups are added up through shared memory, in order, and the CTA writes one row of partial sums (the gradients
@@ -697,18 +716,19 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
                 dbias[q] = dbias[q] + Two<A>(__shfl_xor_sync(0xffffffffu, b.x, offset), __shfl_xor_sync(0xffffffffu, b.y, offset));
             }
     const int teams = SPAN != 32 ? (int)blockDim.x / 32 : shape.groups;
+    if (teams == 1 && !final) {  // straight to the CTA's partial row
+        store_sums<A, V, K>(partial + place.at, place, dweight, p.cols % 4 == 0);
+        store_sums<A, V, K>(partial + p.cols + place.at, place, dbias, p.cols % 4 == 0);
+        return;
+    }
     const int team = SPAN != 32 ? (int)threadIdx.x / 32 : place.group;
     A* const tile = reinterpret_cast<A*>(dynamic);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();  // the ring is no longer read or written
-    if (SPAN == 32 || (int)(threadIdx.x % 32) < threads)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int c = place.at - place.begin + e / V * place.hop() + e % V;
-            const auto w = dweight[e / 2].both(), b = dbias[e / 2].both();
-            tile[team * 2 * width + c] = e % 2 == 0 ? w.x : w.y;
-            tile[team * 2 * width + width + c] = e % 2 == 0 ? b.x : b.y;
-        }
+    if (SPAN == 32 || (int)(threadIdx.x % 32) < threads) {
+        store_sums<A, V, K>(tile + team * 2 * width + place.at - place.begin, place, dweight, true);
+        store_sums<A, V, K>(tile + team * 2 * width + width + place.at - place.begin, place, dbias, true);
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < place.end - place.begin; c += blockDim.x) {
         A w = tile[c], b = tile[width + c];
@@ -726,33 +746,40 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
     }
 }
 
-// dweight and dbias from the partial rows: COLUMNS columns of one of the two for each CTA, 256 / COLUMNS threads along the
-// rows of each column; added in double in a fixed order.  Few columns (up to 1024) take 8 at a time, so that all loads of a
-// thread are under way at once (128 columns of 296 rows 2 us less than with 32); with many, 32 read whole lines (8192
-// columns of 148 rows 4 us less than with 8).
-template <typename T, int COLUMNS>
+// dweight and dbias from the partial rows: 8 threads across the columns of one of the two, W columns each (16 bytes where
+// the rows allow), 32 threads along the rows, so that all loads of a thread are under way at once; added in double in a
+// fixed order.
+template <typename T, int W>
 __global__ void __launch_bounds__(256) norm_join_kernel(const __grid_constant__ NormBackwardArgs p, int partials) {
     using A = typename Accumulator<T>::type;
-    constexpr int LANES = 256 / COLUMNS;
-    __shared__ double sums[8][COLUMNS];
-    const int column = threadIdx.x % COLUMNS, lane = threadIdx.x / COLUMNS, c = blockIdx.x * COLUMNS + column;
+    __shared__ double sums[8][8 * W];
+    const int across = threadIdx.x % 8, lane = threadIdx.x / 8, c = (blockIdx.x * 8 + across) * W;
     void* out = blockIdx.y == 0 ? p.dweight : p.dbias;
     if (out == nullptr) return;
     const A* partial = static_cast<const A*>(p.partial) + (long long)blockIdx.y * p.cols + c;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial rows are there
-    double sum = 0.0;
+    double sum[W] = {};
     if (c < p.cols) {
 #pragma unroll 10
-        for (int r = lane; r < partials; r += LANES) sum += (double)partial[(long long)r * 2 * p.cols];
+        for (int r = lane; r < partials; r += 32) {
+            const Pack<A, W> part = *reinterpret_cast<const Pack<A, W>*>(partial + (long long)r * 2 * p.cols);
+#pragma unroll
+            for (int i = 0; i < W; ++i) sum[i] += (double)part.v[i];
+        }
     }
 #pragma unroll
-    for (int offset = COLUMNS; offset < 32; offset *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-    if (threadIdx.x % 32 < COLUMNS) sums[threadIdx.x / 32][column] = sum;
+    for (int i = 0; i < W; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 8);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
+        if (threadIdx.x % 32 < 8) sums[threadIdx.x / 32][across * W + i] = sum[i];
+    }
     __syncthreads();
-    if (threadIdx.x >= COLUMNS || c >= p.cols) return;
+    const int column = blockIdx.x * 8 * W + threadIdx.x;
+    if (threadIdx.x >= 8 * W || column >= p.cols) return;
+    double total = sums[0][threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) sum += sums[w][column];
-    store_gradient<T>(out, p.params_f32, c, (A)sum);
+    for (int w = 1; w < 8; ++w) total += sums[w][threadIdx.x];
+    store_gradient<T>(out, p.params_f32, column, (A)total);
 }
 
 // Elements [low, high) of a pack, the others as zeros.
@@ -899,7 +926,9 @@ cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
     if (e == cudaSuccess) e = launch_rows(kernel, (unsigned)(partials * s.cluster), threads, each * threads, s.cluster, stream, a, s);
     if (e != cudaSuccess || partials == 1 || (a.dweight == nullptr && a.dbias == nullptr)) return e;
     cudaLaunchConfig_t config{};
-    const int columns = a.cols <= 1024 ? 8 : 32;
+    constexpr int W = 16 / sizeof(A);
+    const bool vectors = a.cols % W == 0;
+    const int columns = vectors ? 8 * W : 8;
     config.gridDim = dim3((a.cols + columns - 1) / columns, 2);
     config.blockDim = dim3(256);
     config.stream = stream;
@@ -908,7 +937,7 @@ cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
     attribute.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, columns == 8 ? norm_join_kernel<T, 8> : norm_join_kernel<T, 32>, a, partials);
+    return cudaLaunchKernelEx(&config, vectors ? norm_join_kernel<T, W> : norm_join_kernel<T, 1>, a, partials);
 }
 
 template <typename T>
