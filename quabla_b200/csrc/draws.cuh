@@ -54,10 +54,12 @@ struct DrawStream {
         return state + (unsigned long long)(((index + odd) >> 1) + 1) * GAMMA;
     }
     __device__ __forceinline__ unsigned int half(long long index) const { return ((unsigned int)index + odd) & 1u; }
-    __device__ __forceinline__ bool kept(long long index) const {
-        const unsigned long long z = mix(at(index)), bits = z ^ (z >> 31);
-        return (half(index) ? (unsigned int)(bits >> 32) : (unsigned int)bits) >= threshold;
+    // One half of the word at a state, and one element.
+    __device__ __forceinline__ bool kept_half(unsigned long long at, bool high) const {
+        const unsigned long long z = mix(at), bits = z ^ (z >> 31);
+        return (high ? (unsigned int)(bits >> 32) : (unsigned int)bits) >= threshold;
     }
+    __device__ __forceinline__ bool kept(long long index) const { return kept_half(at(index), half(index) != 0); }
 };
 
 }  // namespace qb

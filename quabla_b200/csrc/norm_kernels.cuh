@@ -17,6 +17,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "norm.h"
@@ -283,26 +284,48 @@ template <typename T, int V, int ARRAYS, int ROWS, int STAGES> struct RowRing {
     static __device__ __forceinline__ Pack<T, V>* at(char* stage, int r, int array, int k) {
         return reinterpret_cast<Pack<T, V>*>(stage + ((r * ARRAYS + array) * K + k) * 32 * BYTES);
     }
+    // Pack k of an array: all of it, or its first `count` elements (none for a row that is not there).
     static __device__ __forceinline__ void fetch(char* stage, int r, int array, int k, const T* from) {
-        if constexpr (BYTES >= 4) {
-            const unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, r, array, k));
-            if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-            else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES < 4 ? 4 : BYTES) : "memory");
-        } else {
-            at(stage, r, array, k)->v[0] = *from;
-        }
+        const unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, r, array, k));
+        if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
     }
-    // `count` elements at `from`: a whole pack, less at a row's end, none for a row that is not there.
     static __device__ __forceinline__ void fetch(char* stage, int r, int array, int k, const T* from, int count) {
-        if constexpr (BYTES >= 4) {
-            const unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, r, array, k));
-            const int bytes = count * (int)sizeof(T);
-            if constexpr (BYTES == 16)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-            else
-                asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES < 4 ? 4 : BYTES), "r"(bytes) : "memory");
+        const unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, r, array, k));
+        const int bytes = count * (int)sizeof(T);
+        if constexpr (BYTES == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+        else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
+    }
+    // Row r of a turn: a thread's packs of all arrays, the last one of which may be absent.
+    template <typename P>
+    static __device__ __forceinline__ void fetch_row(char* stage, int r, const T* const (&from)[ARRAYS], bool last, const P& place, bool there) {
+        if constexpr (BYTES < 4) {  // no asynchronous copy is that small: all loads first, then all stores
+            T v[ARRAYS][K];
+#pragma unroll
+            for (int a = 0; a < ARRAYS; ++a)
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    v[a][k] = there && place.count(k) > 0 && (last || a < ARRAYS - 1) ? from[a][k * place.hop()] : narrow<T>((typename Accumulator<T>::type)0);
+#pragma unroll
+            for (int a = 0; a < ARRAYS; ++a)
+#pragma unroll
+                for (int k = 0; k < K; ++k) at(stage, r, a, k)->v[0] = v[a][k];
+        } else if (there && place.whole()) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int a = 0; a < ARRAYS; ++a)
+                    if (last || a < ARRAYS - 1) fetch(stage, r, a, k, from[a] + k * place.hop());
         } else {
-            at(stage, r, array, k)->v[0] = count > 0 ? *from : narrow<T>((typename Accumulator<T>::type)0);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int count = there ? place.count(k) : 0;
+#pragma unroll
+                for (int a = 0; a < ARRAYS; ++a)
+                    if (last || a < ARRAYS - 1) fetch(stage, r, a, k, from[a] + k * place.hop(), count);
+            }
         }
     }
     // A thread's packs of a row as pairs.
@@ -381,10 +404,16 @@ __device__ __forceinline__ void drop(const DrawStream& draws, long long index, i
     if constexpr (D == Draws::NONE) {
         return;
     } else if constexpr (V == 1) {
+        // An even number of columns apart, a thread's elements are the same halves of words a constant apart.
+        const unsigned long long first = draws.at(index);
+        const bool even = hop % 2 == 0, high = draws.half(index) != 0;
+        auto kept = [&](int k) {
+            return even ? draws.kept_half(first + (unsigned long long)(k * (hop / 2)) * DrawStream::GAMMA, high) : draws.kept(index + k * hop);
+        };
 #pragma unroll
         for (int k = 0; k < PACKS; k += 2) {
             const auto f = (pairs[k / 2] * Two<A>(scale)).both();
-            pairs[k / 2] = Two<A>(draws.kept(index + k * hop) ? f.x : (A)0, draws.kept(index + (k + 1) * hop) ? f.y : (A)0);
+            pairs[k / 2] = Two<A>(kept(k) ? f.x : (A)0, kept(k + 1) ? f.y : (A)0);
         }
     } else if constexpr (D == Draws::PLAIN) {
         drop_from_low<V, PACKS, false>(draws, index, hop, scale, pairs);
@@ -415,7 +444,7 @@ template <typename T, int V, int SPAN, bool RESIDUAL>
 __global__ void __maxnreg__(128)
 norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
-    constexpr int ARRAYS = RESIDUAL ? 2 : 1, R = norm_forward_rows(sizeof(T), V > 1), STAGES = norm_forward_stages(sizeof(T), V > 1, RESIDUAL);
+    constexpr int ARRAYS = RESIDUAL ? 2 : 1, R = norm_forward_rows(sizeof(T), V * sizeof(T) == 16), STAGES = norm_forward_stages(sizeof(T), V * sizeof(T) == 16, RESIDUAL);
     using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
     __shared__ typename RowSum<A, R, SPAN>::Shared shared;
@@ -433,22 +462,10 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
     auto fetch = [&](char* stage, int turn) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const T* from = x + r * p.x.stride;
-            const T* more = residual + r * p.residual.stride;
-            if (whole && turn < place.there[r]) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    ring.fetch(stage, r, 0, k, from + k * place.hop());
-                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, more + k * place.hop());
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const int count = turn < place.there[r] ? place.count(k) : 0;
-                    ring.fetch(stage, r, 0, k, from + k * place.hop(), count);
-                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, more + k * place.hop(), count);
-                }
-            }
+            const T* from[ARRAYS];
+            if (RESIDUAL) from[ARRAYS - 1] = residual + r * p.residual.stride;
+            from[0] = x + r * p.x.stride;
+            ring.fetch_row(stage, r, from, !RESIDUAL || added, place, turn < place.there[r]);
         }
         ring.commit();
         x += p.x.advance;
@@ -574,7 +591,7 @@ template <typename T, int V, int SPAN, bool RESIDUAL>
 __global__ void __maxnreg__(128)
 norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
-    constexpr int ARRAYS = RESIDUAL ? 3 : 2, R = norm_backward_rows(sizeof(T), V > 1, SPAN == 32), STAGES = norm_backward_stages(RESIDUAL);
+    constexpr int ARRAYS = RESIDUAL ? 3 : 2, R = norm_backward_rows(sizeof(T), V * sizeof(T) == 16, SPAN == 32), STAGES = norm_backward_stages(RESIDUAL);
     using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
     __shared__ typename RowSum<A, 2 * R, SPAN>::Shared shared;
@@ -593,23 +610,11 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
     auto fetch = [&](char* stage, int turn) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const T* from[3] = {dy + r * p.dy.stride, h + r * p.h.stride, dh + r * p.dh.stride};
-            if (whole && turn < place.there[r]) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    ring.fetch(stage, r, 0, k, from[0] + k * place.hop());
-                    ring.fetch(stage, r, 1, k, from[1] + k * place.hop());
-                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, from[2] + k * place.hop());
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const int count = turn < place.there[r] ? place.count(k) : 0;
-                    ring.fetch(stage, r, 0, k, from[0] + k * place.hop(), count);
-                    ring.fetch(stage, r, 1, k, from[1] + k * place.hop(), count);
-                    if (added) ring.fetch(stage, r, ARRAYS - 1, k, from[2] + k * place.hop(), count);
-                }
-            }
+            const T* from[ARRAYS];
+            if (RESIDUAL) from[ARRAYS - 1] = dh + r * p.dh.stride;
+            from[0] = dy + r * p.dy.stride;
+            from[1] = h + r * p.h.stride;
+            ring.fetch_row(stage, r, from, !RESIDUAL || added, place, turn < place.there[r]);
         }
         ring.commit();
         dy += p.dy.advance;
@@ -868,9 +873,21 @@ __global__ void __launch_bounds__(256, ONE_ROW ? 4 : 6) dropout_kernel(const __g
 
 // ---- launches ----------------------------------------------------------------------------------
 
-// Whether rows start on 16-byte boundaries, so that a thread can take 16 bytes at a time.
-inline bool rows_aligned(const RowArray& a, long long rows, size_t element) {
-    return reinterpret_cast<uintptr_t>(a.data) % 16 == 0 && (rows <= 1 || a.stride * element % 16 == 0);
+// Whether rows start on boundaries of `bytes`, so that a thread can take that much at a time.
+inline bool rows_aligned(const RowArray& a, long long rows, size_t element, size_t bytes) {
+    return reinterpret_cast<uintptr_t>(a.data) % bytes == 0 && (rows <= 1 || a.stride * element % bytes == 0);
+}
+
+// Elements that are taken at a time: 16 bytes, 4 bytes of 16-bit rows (even strides that are no multiple of 8), or one.
+template <typename T>
+int pack_of(std::initializer_list<const RowArray*> arrays, long long rows) {
+    for (const size_t bytes : {size_t(16), size_t(4)}) {
+        if (bytes <= sizeof(T)) break;
+        bool all = true;
+        for (const RowArray* a : arrays) all = all && rows_aligned(*a, rows, sizeof(T), bytes);
+        if (all) return (int)(bytes / sizeof(T));
+    }
+    return 1;
 }
 
 template <typename... P, typename... Q>
@@ -892,36 +909,42 @@ cudaError_t launch_rows(void (*kernel)(P...), unsigned grid, unsigned threads, s
 template <typename T, int V, bool RESIDUAL>
 cudaError_t launch_forward(NormForwardArgs a, cudaStream_t stream) {
     const RowShape s = row_shape(a.cols, norm_elements(sizeof(T)));
-    const int threads = s.threads_per_row * s.groups, together = s.groups * norm_forward_rows(sizeof(T), V > 1);
+    const int threads = s.threads_per_row * s.groups, together = s.groups * norm_forward_rows(sizeof(T), V * sizeof(T) == 16);
     const long long batches = (a.rows + together - 1) / together, resident = NORM_SMS * (NORM_MAX_THREADS / threads) / s.cluster;
     const long long clusters = std::min(batches, resident);
     for (RowArray* r : {&a.x, &a.residual, &a.h, &a.y}) r->advance = clusters * together * r->stride;
     auto kernel = s.threads_per_row >= 32 ? norm_forward_kernel<T, V, 32, RESIDUAL> : norm_forward_kernel<T, V, 0, RESIDUAL>;
-    const size_t each = norm_forward_shared(sizeof(T), V > 1, RESIDUAL);
+    const size_t each = norm_forward_shared(sizeof(T), V * sizeof(T) == 16, RESIDUAL);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
     return e != cudaSuccess ? e : launch_rows(kernel, (unsigned)(clusters * s.cluster), threads, each * threads, s.cluster, stream, a, s);
 }
 
+template <typename T, bool RESIDUAL>
+cudaError_t launch_forward(const NormForwardArgs& a, cudaStream_t stream) {
+    constexpr int WIDE = 16 / sizeof(T);
+    const int pack = pack_of<T>({&a.x, &a.residual, &a.h, &a.y}, a.rows);
+    if (pack == WIDE) return launch_forward<T, WIDE, RESIDUAL>(a, stream);
+    if constexpr (sizeof(T) == 2)
+        if (pack == 2) return launch_forward<T, 2, RESIDUAL>(a, stream);
+    return launch_forward<T, 1, RESIDUAL>(a, stream);
+}
+
 template <typename T>
 cudaError_t norm_forward_launch(const NormForwardArgs& a, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = rows_aligned(a.x, a.rows, sizeof(T)) && rows_aligned(a.residual, a.rows, sizeof(T)) &&
-                      rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.y, a.rows, sizeof(T));
-    if (a.residual.data != nullptr || a.h.data != nullptr || a.draw.active)
-        return wide ? launch_forward<T, V, true>(a, stream) : launch_forward<T, 1, true>(a, stream);
-    return wide ? launch_forward<T, V, false>(a, stream) : launch_forward<T, 1, false>(a, stream);
+    const bool residual = a.residual.data != nullptr || a.h.data != nullptr || a.draw.active;
+    return residual ? launch_forward<T, true>(a, stream) : launch_forward<T, false>(a, stream);
 }
 
 template <typename T, int V, bool RESIDUAL>
 cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
     using A = typename Accumulator<T>::type;
     const RowShape s = row_shape(a.cols, norm_elements(sizeof(T)));
-    const int threads = s.threads_per_row * s.groups, rows_at_once = norm_backward_rows(sizeof(T), V > 1, s.threads_per_row >= 32);
+    const int threads = s.threads_per_row * s.groups, rows_at_once = norm_backward_rows(sizeof(T), V * sizeof(T) == 16, s.threads_per_row >= 32);
     const int partials = norm_partials(a.rows, rows_at_once, s);
     for (RowArray* r : {&a.dy, &a.dh, &a.h, &a.dx, &a.dresidual}) r->advance = (long long)partials * s.groups * rows_at_once * r->stride;
     auto kernel = s.threads_per_row >= 32 ? norm_backward_kernel<T, V, 32, RESIDUAL> : norm_backward_kernel<T, V, 0, RESIDUAL>;
     // The ring's space later holds the groups' shares of the parameters' gradients: two values for each element.
-    const size_t each = std::max(norm_backward_shared(sizeof(T), V > 1, s.threads_per_row >= 32, RESIDUAL), 2 * norm_elements(sizeof(T)) * sizeof(A));
+    const size_t each = std::max(norm_backward_shared(sizeof(T), V * sizeof(T) == 16, s.threads_per_row >= 32, RESIDUAL), 2 * norm_elements(sizeof(T)) * sizeof(A));
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
     if (e == cudaSuccess) e = launch_rows(kernel, (unsigned)(partials * s.cluster), threads, each * threads, s.cluster, stream, a, s);
     if (e != cudaSuccess || partials == 1 || (a.dweight == nullptr && a.dbias == nullptr)) return e;
@@ -940,15 +963,20 @@ cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
     return cudaLaunchKernelEx(&config, vectors ? norm_join_kernel<T, W> : norm_join_kernel<T, 1>, a, partials);
 }
 
+template <typename T, bool RESIDUAL>
+cudaError_t launch_backward(const NormBackwardArgs& a, cudaStream_t stream) {
+    constexpr int WIDE = 16 / sizeof(T);
+    const int pack = pack_of<T>({&a.dy, &a.dh, &a.h, &a.dx, &a.dresidual}, a.rows);
+    if (pack == WIDE) return launch_backward<T, WIDE, RESIDUAL>(a, stream);
+    if constexpr (sizeof(T) == 2)
+        if (pack == 2) return launch_backward<T, 2, RESIDUAL>(a, stream);
+    return launch_backward<T, 1, RESIDUAL>(a, stream);
+}
+
 template <typename T>
 cudaError_t norm_backward_launch(const NormBackwardArgs& a, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = rows_aligned(a.dy, a.rows, sizeof(T)) && rows_aligned(a.dh, a.rows, sizeof(T)) &&
-                      rows_aligned(a.h, a.rows, sizeof(T)) && rows_aligned(a.dx, a.rows, sizeof(T)) &&
-                      rows_aligned(a.dresidual, a.rows, sizeof(T));
-    if (a.dh.data != nullptr || a.dresidual.data != nullptr || a.draw.active)
-        return wide ? launch_backward<T, V, true>(a, stream) : launch_backward<T, 1, true>(a, stream);
-    return wide ? launch_backward<T, V, false>(a, stream) : launch_backward<T, 1, false>(a, stream);
+    const bool residual = a.dh.data != nullptr || a.dresidual.data != nullptr || a.draw.active;
+    return residual ? launch_backward<T, true>(a, stream) : launch_backward<T, false>(a, stream);
 }
 
 template <typename T>

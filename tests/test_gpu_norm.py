@@ -18,6 +18,8 @@ pytestmark = pytest.mark.gpu
 SHAPES = [(1, 1, 0, 0), (3, 7, 0, 0), (5, 16, 0, 0), (2, 33, 0, 1), (300, 64, 0, 0), (37, 257, 0, 0), (9, 100, 4, 0), (10, 250, 6, 0),
           (4, 1001, 6, 0), (2, 1001, 7, 0), (513, 48, 16, 0), (3, 4096, 0, 0), (2, 5120, 0, 3), (2, 8200, 0, 0), (1, 50001, 0, 0),
           (2, 20008, 8, 0), (20000, 3, 0, 0), (4099, 130, 0, 0)]
+# 16-bit rows that start on 4-byte boundaries and no wider ones.
+SHAPES += [(300, 34, 0, 0), (6, 250, 0, 0), (37, 1002, 0, 2), (2, 4098, 0, 0), (5, 18, 4, 2)]
 
 
 def shapes_for(dtype):
