@@ -426,10 +426,10 @@ qb200_status qb200_weight_gradient_static(int32_t dtype, const void* d_acts, con
  * row's elements next to each other, row r at data + r * stride elements.
  * Strides of arrays that are read are >= 0 (0 repeats one row), of arrays that
  * are written >= cols; with one row the stride is not looked at.  Pointers need
- * the alignment of one element.  Layer norm reads and writes 16 bytes at a time
- * where the rows of every array of a call start on 16-byte boundaries, dropout
- * where the rows of x and y start at the same distance from one; elsewhere they
- * go one element at a time.  What lies between cols and the stride is neither
+ * the alignment of one element.  Layer norm reads and writes 16 bytes or two
+ * elements at a time where the rows of every array of a call start on boundaries
+ * of that, dropout 16 bytes where the rows of x and y start at the same distance
+ * from such a boundary; elsewhere they go one element at a time.  What lies between cols and the stride is neither
  * read nor written.  Zero rows are valid (the sums over rows are then zero).  Parameters
  * (weight, bias and their gradients) are of `param_dtype`: the rows' dtype, or
  * QB200_F32 beside 16-bit rows; either may be NULL and then stands for 1 or 0.

@@ -38,8 +38,10 @@ qb200_status check_param_dtype(const char* op, int32_t dtype, int32_t param_dtyp
 }
 
 qb200_status check_extents(const char* op, int64_t rows, int64_t cols) {
-    if (rows < 0 || cols < 1) return fail(QB200_INVALID, "%s needs rows >= 0 and cols >= 1; got %lld x %lld", op, (long long)rows, (long long)cols);
-    if (rows > 0 && cols > (int64_t(1) << 56) / rows) return fail(QB200_TOO_LARGE, "%s: %lld x %lld elements", op, (long long)rows, (long long)cols);
+    if (rows < 0 || cols < 1)
+        return fail(QB200_INVALID, "%s needs rows >= 0 and cols >= 1; got %lld x %lld", op, (long long)rows, (long long)cols);
+    if (rows > 0 && cols > (int64_t(1) << 56) / rows)
+        return fail(QB200_TOO_LARGE, "%s: %lld x %lld elements", op, (long long)rows, (long long)cols);
     return QB200_OK;
 }
 
@@ -57,7 +59,8 @@ qb200_status check_rows(const char* op, const char* name, const void* data, int6
     if (reinterpret_cast<uintptr_t>(data) % element_bytes(dtype) != 0)
         return fail(QB200_INVALID, "%s: %s is not aligned to its elements", op, name);
     if (rows > 1 && (stride < (written ? cols : 0) || stride > (int64_t(1) << 56) / rows))
-        return fail(QB200_INVALID, "%s: %s has a row stride of %lld elements for %lld columns", op, name, (long long)stride, (long long)cols);
+        return fail(QB200_INVALID, "%s: %s has a row stride of %lld elements for %lld columns", op, name, (long long)stride,
+                    (long long)cols);
     return QB200_OK;
 }
 
@@ -69,7 +72,8 @@ qb200_status check_present(const char* op, std::initializer_list<Named> arrays) 
 
 qb200_status check_aligned(const char* op, std::initializer_list<Named> arrays, size_t bytes) {
     for (const Named& a : arrays)
-        if (reinterpret_cast<uintptr_t>(a.data) % bytes != 0) return fail(QB200_INVALID, "%s: %s is not aligned to its elements", op, a.name);
+        if (reinterpret_cast<uintptr_t>(a.data) % bytes != 0)
+            return fail(QB200_INVALID, "%s: %s is not aligned to its elements", op, a.name);
     return QB200_OK;
 }
 
@@ -191,7 +195,8 @@ qb200_status run_backward(const char* op, int32_t dtype, int32_t param_dtype, qb
         if (d_workspace == nullptr || workspace_bytes < needed)
             return fail(QB200_INVALID, "%s needs a workspace of %zu bytes for %lld rows of %d, got %zu", op, needed, (long long)rows,
                         cols, d_workspace == nullptr ? (size_t)0 : workspace_bytes);
-        if (reinterpret_cast<uintptr_t>(d_workspace) % 16 != 0) return fail(QB200_INVALID, "%s: the workspace is not aligned to 16 bytes", op);
+        if (reinterpret_cast<uintptr_t>(d_workspace) % 16 != 0)
+            return fail(QB200_INVALID, "%s: the workspace is not aligned to 16 bytes", op);
     }
     a.weight = d_weight;
     a.mean = d_mean;

@@ -6,10 +6,14 @@
 //             dh' = rstd * (g - mean(g) - xh * mean(g * xh)) + dh;  dx = dropout(dh');
 //             dweight = sum over rows of dy * xh;  dbias = sum over rows of dy
 //
-// A row stays in the registers of its threads between its one read and its one write, so the variance is taken about
-// the mean (two passes over registers, not over memory).  Sums, statistics and gradients are float32 (float64 for
-// float64 rows); the rows' type is rounded to once, on the way out.  Sums run in a fixed order: results repeat bit for
-// bit.
+// A row stays on the SM between its one read and its one write, so the variance is taken about the mean (two passes over
+// registers, not over memory).  Sums, statistics and gradients are float32 (float64 for float64 rows); the rows' type is
+// rounded to once, on the way out.  Sums run in a fixed order: results repeat bit for bit.
+//
+// All of it is bound by memory in principle (4 to 10 bytes of traffic for a 16-bit element against 10 to 30 instructions);
+// what kept the first versions from it was instruction issue and the latency of the rows' sums, so the layout below is about
+// few instructions for an element and rows that are fetched ahead.  Rates are given as a share of the measured copy rate of
+// 6542 GB/s, times are of one B200 with inputs that change from call to call.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -61,12 +65,23 @@ template <> struct Two<double> {
     __device__ __forceinline__ double2 both() const { return v; }
     __device__ __forceinline__ double sum() const { return v.x + v.y; }
 };
-__device__ __forceinline__ Two<float> operator+(Two<float> a, Two<float> b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
-__device__ __forceinline__ Two<float> operator*(Two<float> a, Two<float> b) { asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
-__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v)); return c; }
+__device__ __forceinline__ Two<float> operator+(Two<float> a, Two<float> b) {
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+    return a;
+}
+__device__ __forceinline__ Two<float> operator*(Two<float> a, Two<float> b) {
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+    return a;
+}
+__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v));
+    return c;
+}
 __device__ __forceinline__ Two<double> operator+(Two<double> a, Two<double> b) { return {a.v.x + b.v.x, a.v.y + b.v.y}; }
 __device__ __forceinline__ Two<double> operator*(Two<double> a, Two<double> b) { return {a.v.x * b.v.x, a.v.y * b.v.y}; }
-__device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) { return {::fma(a.v.x, b.v.x, c.v.x), ::fma(a.v.y, b.v.y, c.v.y)}; }
+__device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) {
+    return {::fma(a.v.x, b.v.x, c.v.x), ::fma(a.v.y, b.v.y, c.v.y)};
+}
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
@@ -103,27 +118,18 @@ __device__ __forceinline__ Pack<T, V> narrow_pack(const Two<A> (&pairs)[H], int 
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
             const auto f = pairs[(k * V + i) / 2].both();
-            if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(&out.v[i]) = __float22half2_rn(f);
-            else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(&out.v[i]) = __float22bfloat162_rn(f);
-            else out.v[i] = narrow<T>(f.x), out.v[i + 1] = narrow<T>(f.y);
+            if constexpr (std::is_same<T, __half>::value)
+                *reinterpret_cast<__half2*>(&out.v[i]) = __float22half2_rn(f);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+                *reinterpret_cast<__nv_bfloat162*>(&out.v[i]) = __float22bfloat162_rn(f);
+            else
+                out.v[i] = narrow<T>(f.x), out.v[i + 1] = narrow<T>(f.y);
         }
     }
     return out;
 }
 
 // The first `count` elements of a pack.
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* from, int count) {
-    Pack<T, V> p;
-    if (count >= V) {
-        p = *reinterpret_cast<const Pack<T, V>*>(from);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) p.v[i] = i < count ? from[i] : narrow<T>((typename Accumulator<T>::type)0);
-    }
-    return p;
-}
-
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* to, int count, const Pack<T, V>& p) {
     if (count >= V) {
@@ -143,7 +149,8 @@ __device__ __forceinline__ A load_param(const void* params, bool f32, int c) {
 // How a thread finds its place.  SPAN is 32 where a row has one or more whole warps, each with 32 * E columns of its own
 // one behind the other; 0 where several rows share a warp (threads_per_row is then a power of two below 32).  Pack k of a
 // thread starts at column `at` + k * hop.  With whole warps every distance within a thread's packs and slots is a
-// constant of the instruction: with distances from the launch instead the kernels issued half as many instructions again.
+// constant of the instruction: with distances from the launch instead the kernels issued half as many instructions again
+// (8192 x 4096 bfloat16 forward: 22 against 13 million warp instructions, 40 against 30 us at that step).
 template <typename T, int V, int SPAN, int ROWS> struct Place {
     static constexpr int E = norm_elements(sizeof(T)), K = E / V;
     int t, group, rank, begin, end, at;
@@ -300,14 +307,17 @@ template <typename T, int V, int ARRAYS, int ROWS, int STAGES> struct RowRing {
     }
     // Row r of a turn: a thread's packs of all arrays, the last one of which may be absent.
     template <typename P>
-    static __device__ __forceinline__ void fetch_row(char* stage, int r, const T* const (&from)[ARRAYS], bool last, const P& place, bool there) {
+    static __device__ __forceinline__ void fetch_row(char* stage, int r, const T* const (&from)[ARRAYS], bool last, const P& place,
+                                                     bool there) {
         if constexpr (BYTES < 4) {  // no asynchronous copy is that small: all loads first, then all stores
             T v[ARRAYS][K];
 #pragma unroll
             for (int a = 0; a < ARRAYS; ++a)
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    v[a][k] = there && place.count(k) > 0 && (last || a < ARRAYS - 1) ? from[a][k * place.hop()] : narrow<T>((typename Accumulator<T>::type)0);
+                for (int k = 0; k < K; ++k) {
+                    const bool present = there && place.count(k) > 0 && (last || a < ARRAYS - 1);
+                    v[a][k] = present ? from[a][k * place.hop()] : narrow<T>((typename Accumulator<T>::type)0);
+                }
 #pragma unroll
             for (int a = 0; a < ARRAYS; ++a)
 #pragma unroll
@@ -357,7 +367,7 @@ __device__ __forceinline__ void load_columns(const P& place, const void* params,
 
 // How a kernel draws: not at all; PLAIN where every pack starts with the low half of a word (even columns and counter) and
 // no half is flipped; ANY otherwise.  The plain draws are straight code, which the compiler spreads over the waits of what is
-// around them (8192 x 5120 bfloat16, the residual form's gradient: 99 us, with the branches of ANY 104).
+// around them (5 of 104 us of the residual form's gradient at 8192 x 5120 bfloat16).
 enum class Draws { NONE, PLAIN, ANY };
 template <Draws D> using DrawsTag = std::integral_constant<Draws, D>;
 template <int V>
@@ -408,7 +418,8 @@ __device__ __forceinline__ void drop(const DrawStream& draws, long long index, i
         const unsigned long long first = draws.at(index);
         const bool even = hop % 2 == 0, high = draws.half(index) != 0;
         auto kept = [&](int k) {
-            return even ? draws.kept_half(first + (unsigned long long)(k * (hop / 2)) * DrawStream::GAMMA, high) : draws.kept(index + k * hop);
+            return even ? draws.kept_half(first + (unsigned long long)(k * (hop / 2)) * DrawStream::GAMMA, high)
+                        : draws.kept(index + k * hop);
         };
 #pragma unroll
         for (int k = 0; k < PACKS; k += 2) {
@@ -440,11 +451,17 @@ __device__ __forceinline__ void by_draws(const DrawStream& draws, int cols, F&& 
 }
 
 // RESIDUAL: x passes through dropout and may be added to a residual; otherwise h = x.
+// 8192 x 4096 bfloat16: 26.7 us, 77 % (32768 rows: 88 us, 92 %: launch and first rows are 4 us); float32 45 us, 91 %.  The
+// residual form of 4096 x 4096 bfloat16 32 us, 64 %, 28.5 without dropout: the draws are 9 integer instructions an element
+// and 16 warps an SM do not hide all of them.  More warps with fewer registers, parameters in shared memory, and draws for
+// the next turn during this one's sums all measured slower or the same.
 template <typename T, int V, int SPAN, bool RESIDUAL>
 __global__ void __maxnreg__(128)
 norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
-    constexpr int ARRAYS = RESIDUAL ? 2 : 1, R = norm_forward_rows(sizeof(T), V * sizeof(T) == 16), STAGES = norm_forward_stages(sizeof(T), V * sizeof(T) == 16, RESIDUAL);
+    constexpr bool WIDE = V * sizeof(T) == 16;
+    constexpr int ARRAYS = RESIDUAL ? 2 : 1, R = norm_forward_rows(sizeof(T), WIDE);
+    constexpr int STAGES = norm_forward_stages(sizeof(T), WIDE, RESIDUAL);
     using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
     __shared__ typename RowSum<A, R, SPAN>::Shared shared;
@@ -587,11 +604,16 @@ __device__ __forceinline__ void store_sums(A* at, const P& place, const Two<A> (
 // Threads keep their columns' share of dweight and dbias in registers over all rows of the CTA; at the end the CTA's
 // groups are added up through shared memory, in order, and the CTA writes one row of partial sums (the gradients
 // themselves where there is only one).
+// 262144 x 128 float32: 70 us with the joining kernel, 88 % (63 without the parameters' gradients); 8192 x 8192 bfloat16 72 to
+// 76 us, 81 to 86 %.  The residual form at 8192 x 5120 bfloat16 96 us, 67 %, 76 without dropout: rows of 4097 to 5120 columns
+// take 320 threads of the 512 that fit an SM's registers, too few warps to hide the draws.  Clusters of two CTAs for such
+// rows, one row at a time with 96 registers, and masks drawn before the sums measured slower.
 template <typename T, int V, int SPAN, bool RESIDUAL>
 __global__ void __maxnreg__(128)
 norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape shape) {
     using A = typename Accumulator<T>::type;
-    constexpr int ARRAYS = RESIDUAL ? 3 : 2, R = norm_backward_rows(sizeof(T), V * sizeof(T) == 16, SPAN == 32), STAGES = norm_backward_stages(RESIDUAL);
+    constexpr bool WIDE = V * sizeof(T) == 16;
+    constexpr int ARRAYS = RESIDUAL ? 3 : 2, R = norm_backward_rows(sizeof(T), WIDE, SPAN == 32), STAGES = norm_backward_stages(RESIDUAL);
     using Ring = RowRing<T, V, ARRAYS, R, STAGES>;
     constexpr int E = Ring::E, K = Ring::K;
     __shared__ typename RowSum<A, 2 * R, SPAN>::Shared shared;
@@ -815,9 +837,12 @@ __device__ __forceinline__ void drop_packs(const DrawStream& draws, long long in
 // start at the same distance from one (V > 1): pack i of a row holds columns [i * V - shift, (i + 1) * V - shift).  One
 // long row (what a contiguous array is) and many rows are two kernels: in the one row the four packs that a thread has on
 // their way are a constant distance apart in the stream of words; of many rows a thread has two.
+// 16384 x 8192 bfloat16: 108 us, 76 %: the integer units are 71 % busy (11 of 17.5 instructions for an element, 4 bytes of
+// traffic); 8192 x 8192 float32 86 us, 95 %.
 __host__ __device__ constexpr int dropout_depth(bool one_row) { return one_row ? 4 : 2; }
 template <typename T, int V, bool ONE_ROW>
-__global__ void __launch_bounds__(256, ONE_ROW ? 4 : 6) dropout_kernel(const __grid_constant__ DropoutArgs p, long long packs, long long packs_per_row) {
+__global__ void __launch_bounds__(256, ONE_ROW ? 4 : 6)
+dropout_kernel(const __grid_constant__ DropoutArgs p, long long packs, long long packs_per_row) {
     using A = typename Accumulator<T>::type;
     constexpr int DEPTH = dropout_depth(ONE_ROW);
     const DrawStream draws(p.draw);
@@ -845,7 +870,8 @@ __global__ void __launch_bounds__(256, ONE_ROW ? 4 : 6) dropout_kernel(const __g
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             const long long pack = first + (long long)d * hop;
-            row[d] = ONE_ROW ? 0 : packs <= 0xffffffffll ? (long long)((unsigned int)pack / (unsigned int)packs_per_row) : pack / packs_per_row;
+            if (ONE_ROW) row[d] = 0;
+            else row[d] = packs <= 0xffffffffll ? (long long)((unsigned int)pack / (unsigned int)packs_per_row) : pack / packs_per_row;
             const T* x = static_cast<const T*>(p.x.data) + row[d] * p.x.stride;
             c[d] = (pack - row[d] * packs_per_row) * V - shift_of(x);
             const long long left = p.cols - c[d];
@@ -892,7 +918,8 @@ int pack_of(std::initializer_list<const RowArray*> arrays, long long rows) {
 }
 
 template <typename... P, typename... Q>
-cudaError_t launch_rows(void (*kernel)(P...), unsigned grid, unsigned threads, size_t shared, int cluster, cudaStream_t stream, const Q&... args) {
+cudaError_t launch_rows(void (*kernel)(P...), unsigned grid, unsigned threads, size_t shared, int cluster, cudaStream_t stream,
+                        const Q&... args) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
@@ -910,12 +937,13 @@ cudaError_t launch_rows(void (*kernel)(P...), unsigned grid, unsigned threads, s
 template <typename T, int V, bool RESIDUAL>
 cudaError_t launch_forward(NormForwardArgs a, cudaStream_t stream) {
     const RowShape s = row_shape(a.cols, norm_elements(sizeof(T)));
-    const int threads = s.threads_per_row * s.groups, together = s.groups * norm_forward_rows(sizeof(T), V * sizeof(T) == 16);
+    constexpr bool WIDE = V * sizeof(T) == 16;
+    const int threads = s.threads_per_row * s.groups, together = s.groups * norm_forward_rows(sizeof(T), WIDE);
     const long long batches = (a.rows + together - 1) / together, resident = NORM_SMS * (NORM_MAX_THREADS / threads) / s.cluster;
     const long long clusters = std::min(batches, resident);
     for (RowArray* r : {&a.x, &a.residual, &a.h, &a.y}) r->advance = clusters * together * r->stride;
     auto kernel = s.threads_per_row >= 32 ? norm_forward_kernel<T, V, 32, RESIDUAL> : norm_forward_kernel<T, V, 0, RESIDUAL>;
-    const size_t each = norm_forward_shared(sizeof(T), V * sizeof(T) == 16, RESIDUAL);
+    const size_t each = norm_forward_shared(sizeof(T), WIDE, RESIDUAL);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
     return e != cudaSuccess ? e : launch_rows(kernel, (unsigned)(clusters * s.cluster), threads, each * threads, s.cluster, stream, a, s);
 }
@@ -940,12 +968,14 @@ template <typename T, int V, bool RESIDUAL>
 cudaError_t launch_backward(NormBackwardArgs a, cudaStream_t stream) {
     using A = typename Accumulator<T>::type;
     const RowShape s = row_shape(a.cols, norm_elements(sizeof(T)));
-    const int threads = s.threads_per_row * s.groups, rows_at_once = norm_backward_rows(sizeof(T), V * sizeof(T) == 16, s.threads_per_row >= 32);
+    constexpr bool WIDE = V * sizeof(T) == 16;
+    const bool whole_warps = s.threads_per_row >= 32;
+    const int threads = s.threads_per_row * s.groups, rows_at_once = norm_backward_rows(sizeof(T), WIDE, whole_warps);
     const int partials = norm_partials(a.rows, rows_at_once, s);
     for (RowArray* r : {&a.dy, &a.dh, &a.h, &a.dx, &a.dresidual}) r->advance = (long long)partials * s.groups * rows_at_once * r->stride;
-    auto kernel = s.threads_per_row >= 32 ? norm_backward_kernel<T, V, 32, RESIDUAL> : norm_backward_kernel<T, V, 0, RESIDUAL>;
+    auto kernel = whole_warps ? norm_backward_kernel<T, V, 32, RESIDUAL> : norm_backward_kernel<T, V, 0, RESIDUAL>;
     // The ring's space later holds the groups' shares of the parameters' gradients: two values for each element.
-    const size_t each = std::max(norm_backward_shared(sizeof(T), V * sizeof(T) == 16, s.threads_per_row >= 32, RESIDUAL), 2 * norm_elements(sizeof(T)) * sizeof(A));
+    const size_t each = std::max(norm_backward_shared(sizeof(T), WIDE, whole_warps, RESIDUAL), 2 * norm_elements(sizeof(T)) * sizeof(A));
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(each * NORM_MAX_THREADS));
     if (e == cudaSuccess) e = launch_rows(kernel, (unsigned)(partials * s.cluster), threads, each * threads, s.cluster, stream, a, s);
     if (e != cudaSuccess || partials == 1 || (a.dweight == nullptr && a.dbias == nullptr)) return e;
@@ -996,7 +1026,8 @@ cudaError_t dropout_launch(const DropoutArgs& given, cudaStream_t stream) {
     // units and 8 CTAs for each SM do best (16384 x 8192 bfloat16 108 us, with 24 119), others by memory and 24 (8192 x 8192
     // float32 86 us, with 8 95).
     const long long spread = (packs + 255) / 256, deep = (packs + each - 1) / each;
-    const unsigned grid = (unsigned)(spread <= NORM_SMS * 4 ? spread : std::max<long long>(NORM_SMS * 4, std::min<long long>(deep, NORM_SMS * (sizeof(T) == 2 && a.rows == 1 ? 8 : 24))));
+    const long long most = NORM_SMS * (sizeof(T) == 2 && a.rows == 1 ? 8 : 24), least = NORM_SMS * 4;
+    const unsigned grid = (unsigned)(spread <= least ? spread : std::max(least, std::min(deep, most)));
     auto kernel = a.rows == 1 ? (wide ? dropout_kernel<T, V, true> : dropout_kernel<T, 1, true>)
                               : (wide ? dropout_kernel<T, V, false> : dropout_kernel<T, 1, false>);
     return launch_rows(kernel, grid, 256, 0, 1, stream, a, packs, per_row);
