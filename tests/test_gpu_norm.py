@@ -243,6 +243,35 @@ def test_offsets_past_32_bits(cuda_device, dtype):
     assert (y.view == x.view).all()
 
 
+def test_more_elements_than_31_bits_count(cuda_device):
+    import torch
+
+    lib, n, key, rate = _lib.load(), (1 << 31) + 77, qb.random.key(31), 0.3
+    x = torch.ones(n, dtype=torch.float16, device="cuda")
+    _lib.check(lib.qb200_dropout(_lib.F16, x.data_ptr(), n, 1, n, rate, key.value, 5, None, x.data_ptr(), n, nu.stream()))
+    for first in (0, n - 1000):  # the last thousand lie on both sides of 2^31
+        kept = torch.from_numpy(qb.random.dropout_mask(key, (1000,), rate, 5 + first)).cuda()
+        assert ((x[first:first + 1000] != 0) == kept).all()
+    del x
+    rows, cols = (1 << 28) + 3, 8
+    x = nu.Rows(0, cols, "float16")
+    x.rows, x.view = rows, torch.empty(rows, cols, dtype=torch.float16, device="cuda").normal_()
+    y, mean, rstd = torch.empty_like(x.view), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    out = nu.Rows(0, cols, "float16")
+    out.rows, out.view = rows, y
+    nu.layer_norm("float16", "float16", x, None, None, out, mean, rstd)
+    dx = nu.Rows(0, cols, "float16")
+    dx.rows, dx.view = rows, torch.empty_like(y)
+    nu.layer_norm_backward("float16", "float16", out, x, None, mean, rstd, dx, None, None)
+    for first in (0, (1 << 27) - 7, rows - 1000):
+        part = slice(first, first + 1000)
+        some = nu.Rows(1000, cols, "float16", values=x.view[part])
+        got = nu.Rows(1000, cols, "float16", values=y[part])
+        nu.check_forward("float16", some.wide(), None, None, got, mean[part], rstd[part])
+        nu.check_backward("float16", "float16", got, some, None, mean[part], rstd[part],
+                          nu.Rows(1000, cols, "float16", values=dx.view[part]), None, None)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("rows,cols", [(70, 96), (70, 97), (3, 9000)])
 def test_absent_parameters_and_outputs(cuda_device, dtype, rows, cols):
