@@ -305,23 +305,34 @@ template <typename T, int V, int ARRAYS, int ROWS, int STAGES> struct RowRing {
         else
             asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
     }
-    // Row r of a turn: a thread's packs of all arrays, the last one of which may be absent.
+    // Row r of a turn: a thread's packs of all arrays, the last one of which may be absent.  No asynchronous copy is as small
+    // as one 16-bit element: all loads go before the stores to the slots, and of a single array they wait in registers until
+    // `settle` stores them at the turn's end (8192 x 4095 bfloat16 49 us, otherwise 62; of more arrays the registers spill).
+    static constexpr bool LATE = BYTES < 4 && ARRAYS == 1;
+    struct Pending { T v[BYTES < 4 ? ARRAYS : 1][BYTES < 4 ? K : 1]; };
+    static __device__ __forceinline__ void put(char* stage, int r, const Pending& pending) {
+#pragma unroll
+        for (int a = 0; a < ARRAYS; ++a)
+#pragma unroll
+            for (int k = 0; k < K; ++k) at(stage, r, a, k)->v[0] = pending.v[a][k];
+    }
+    static __device__ __forceinline__ void settle(char* stage, const Pending (&pending)[ROWS]) {
+        if constexpr (LATE)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) put(stage, r, pending[r]);
+    }
     template <typename P>
     static __device__ __forceinline__ void fetch_row(char* stage, int r, const T* const (&from)[ARRAYS], bool last, const P& place,
-                                                     bool there) {
-        if constexpr (BYTES < 4) {  // no asynchronous copy is that small: all loads first, then all stores
-            T v[ARRAYS][K];
+                                                     bool there, Pending& pending) {
+        if constexpr (BYTES < 4) {
 #pragma unroll
             for (int a = 0; a < ARRAYS; ++a)
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const bool present = there && place.count(k) > 0 && (last || a < ARRAYS - 1);
-                    v[a][k] = present ? from[a][k * place.hop()] : narrow<T>((typename Accumulator<T>::type)0);
+                    pending.v[a][k] = present ? from[a][k * place.hop()] : narrow<T>((typename Accumulator<T>::type)0);
                 }
-#pragma unroll
-            for (int a = 0; a < ARRAYS; ++a)
-#pragma unroll
-                for (int k = 0; k < K; ++k) at(stage, r, a, k)->v[0] = v[a][k];
+            if constexpr (!LATE) put(stage, r, pending);
         } else if (there && place.whole()) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -476,20 +487,24 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
     T* h_out = static_cast<T*>(p.h.data) + row * p.h.stride + place.at;
     T* y = static_cast<T*>(p.y.data) + row * p.y.stride + place.at;
 
+    typename Ring::Pending pending[R];
     auto fetch = [&](char* stage, int turn) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const T* from[ARRAYS];
             if (RESIDUAL) from[ARRAYS - 1] = residual + r * p.residual.stride;
             from[0] = x + r * p.x.stride;
-            ring.fetch_row(stage, r, from, !RESIDUAL || added, place, turn < place.there[r]);
+            ring.fetch_row(stage, r, from, !RESIDUAL || added, place, turn < place.there[r], pending[r]);
         }
         ring.commit();
         x += p.x.advance;
         if (RESIDUAL) residual += p.residual.advance;
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch(ring.stage(s), s);
+    for (int s = 0; s < STAGES - 1; ++s) {
+        fetch(ring.stage(s), s);
+        ring.settle(ring.stage(s), pending);
+    }
 
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale, inverse = (A)1 / (A)p.cols;
@@ -501,7 +516,8 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
         const int turns = place.turns(p.rows);
         char *now = ring.stage(0), *free = ring.stage(STAGES - 1);  // the slots in work; those read in the last turn
         for (int turn = 0; turn < turns; ++turn) {
-            fetch(free, turn + STAGES - 1);
+            char* const next = free;
+            fetch(next, turn + STAGES - 1);
             ring.wait();
             Two<A> h[R][E / 2];
             A sum[R];
@@ -567,6 +583,7 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
                     }
                 }
             }
+            ring.settle(next, pending);
             row += place.step;
             y += p.y.advance;
             if (RESIDUAL) h_out += p.h.advance;
@@ -629,6 +646,7 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
     T* dx = static_cast<T*>(p.dx.data) + row * p.dx.stride + place.at;
     T* dresidual = static_cast<T*>(p.dresidual.data) + row * p.dresidual.stride + place.at;
 
+    typename Ring::Pending pending[R];
     auto fetch = [&](char* stage, int turn) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -636,7 +654,7 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
             if (RESIDUAL) from[ARRAYS - 1] = dh + r * p.dh.stride;
             from[0] = dy + r * p.dy.stride;
             from[1] = h + r * p.h.stride;
-            ring.fetch_row(stage, r, from, !RESIDUAL || added, place, turn < place.there[r]);
+            ring.fetch_row(stage, r, from, !RESIDUAL || added, place, turn < place.there[r], pending[r]);
         }
         ring.commit();
         dy += p.dy.advance;
@@ -644,7 +662,10 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
         if (RESIDUAL) dh += p.dh.advance;
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch(ring.stage(s), s);
+    for (int s = 0; s < STAGES - 1; ++s) {
+        fetch(ring.stage(s), s);
+        ring.settle(ring.stage(s), pending);
+    }
 
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale, inverse = (A)1 / (A)p.cols;
@@ -720,6 +741,7 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
                 }
                 if (live) place.store(dx + r * p.dx.stride, d, whole);
             }
+            ring.settle(free, pending);
             free = now;
             now = now == ring.stage(STAGES - 1) ? ring.stage(0) : now + Ring::STAGE_BYTES;
             row += place.step;
@@ -836,7 +858,8 @@ __device__ __forceinline__ void drop_packs(const DrawStream& draws, long long in
 // Dropout alone.  Rows are taken in 16-byte packs from 16-byte boundary to boundary wherever they start, as long as x and y
 // start at the same distance from one (V > 1): pack i of a row holds columns [i * V - shift, (i + 1) * V - shift).  One
 // long row (what a contiguous array is) and many rows are two kernels: in the one row the four packs that a thread has on
-// their way are a constant distance apart in the stream of words; of many rows a thread has two.
+// their way are a constant distance apart in the stream of words; of many rows a thread has two (8192 x 4095 bfloat16 55 us, with
+// four 62).
 // 16384 x 8192 bfloat16: 108 us, 76 %: the integer units are 71 % busy (11 of 17.5 instructions for an element, 4 bytes of
 // traffic); 8192 x 8192 float32 86 us, 95 %.
 __host__ __device__ constexpr int dropout_depth(bool one_row) { return one_row ? 4 : 2; }

@@ -9,8 +9,6 @@ themselves, of the quotients and of what follows, 64 u covers every first-order 
 import ctypes as C
 import math
 
-import numpy as np
-
 from quabla_b200 import _lib
 from quabla_b200 import random as qr
 
@@ -238,10 +236,6 @@ def check_backward(dtype, params, dy, h, weight, mean, rstd, dx, dweight, dbias,
 
 
 def same_bits(a, b):
-    return a.contiguous().cpu().view(-1).numpy().tobytes() == b.contiguous().cpu().view(-1).numpy().tobytes() \
-        if a.dtype.itemsize > 2 else bool((a.contiguous().view(-1).view(__import__("torch").int16)
-                                           == b.contiguous().view(-1).view(__import__("torch").int16)).all())
+    import torch
 
-
-def as_uint64(value):
-    return np.uint64(value & ((1 << 64) - 1))
+    return torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
