@@ -622,7 +622,7 @@ __device__ __forceinline__ void store_sums(A* at, const P& place, const Two<A> (
 // groups are added up through shared memory, in order, and the CTA writes one row of partial sums (the gradients
 // themselves where there is only one).
 // 262144 x 128 float32: 70 us with the joining kernel, 88 % (63 without the parameters' gradients); 8192 x 8192 bfloat16 72 to
-// 76 us, 81 to 86 %.  The residual form at 8192 x 5120 bfloat16 96 us, 67 %, 76 without dropout: rows of 4097 to 5120 columns
+// 78 us, 79 to 86 %.  The residual form at 8192 x 5120 bfloat16 96 us, 67 %, 76 without dropout: rows of 4097 to 5120 columns
 // take 320 threads of the 512 that fit an SM's registers, too few warps to hide the draws.  Clusters of two CTAs for such
 // rows, one row at a time with 96 registers, and masks drawn before the sums measured slower.
 template <typename T, int V, int SPAN, bool RESIDUAL>
