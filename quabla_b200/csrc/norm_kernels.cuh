@@ -213,7 +213,14 @@ template <typename A, int N, int SPAN> struct RowSum {
     int turn = 0;
     __device__ __forceinline__ RowSum(Shared& s, const RowShape& shape)
         : shared(s), threads_per_row(shape.threads_per_row), cluster(shape.cluster), lane(threadIdx.x % 32), warp(threadIdx.x / 32),
-          warps(shape.threads_per_row / 32), group(threadIdx.x / shape.threads_per_row) {}
+          warps(shape.threads_per_row / 32), group(threadIdx.x / shape.threads_per_row) {
+        if (SPAN == 32 && cluster > 1) cooperative_groups::this_cluster().barrier_arrive();
+    }
+    // Before the first sum: the shared memory of a cluster's other CTAs may be written only once they run.  Every thread
+    // has arrived when it entered the kernel, so the wait lies under the first rows' copies.
+    __device__ __forceinline__ void meet() const {
+        if (SPAN == 32 && cluster > 1) cooperative_groups::this_cluster().barrier_wait();
+    }
 
     __device__ __forceinline__ void operator()(A (&v)[N]) {
         if constexpr (SPAN == 32) {
@@ -512,6 +519,7 @@ norm_forward_kernel(const __grid_constant__ NormForwardArgs p, const RowShape sh
     load_columns<T, V>(place, p.weight, p.params_f32, (A)1, weight);
     load_columns<T, V>(place, p.bias, p.params_f32, (A)0, bias);
 
+    row_sum.meet();
     by_draws<V, RESIDUAL>(draws, p.cols, [&](auto how) {
         const int turns = place.turns(p.rows);
         char *now = ring.stage(0), *free = ring.stage(STAGES - 1);  // the slots in work; those read in the last turn
@@ -687,6 +695,7 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
         rstds += place.step;
     };
     fetch_statistics(0);
+    row_sum.meet();
     by_draws<V, RESIDUAL>(draws, p.cols, [&](auto how) {
         const int turns = place.turns(p.rows);
         char *now = ring.stage(0), *free = ring.stage(STAGES - 1);
