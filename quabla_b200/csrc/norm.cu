@@ -134,7 +134,11 @@ qb200_status finish(const char* op, cudaError_t e) {
      : (dtype) == QB200_F16 ? qb::launch<__half>(args, stream)                      \
                             : qb::launch<__nv_bfloat16>(args, stream))
 
-qb::RowArray rows_of(const void* data, int64_t stride) { return {const_cast<void*>(data), (long long)stride, 0}; }
+// One row's stride is not looked at, whatever it is: no address is formed with it.  (Groups and turns without a row name a
+// source in their copies of no bytes; it has to be aligned all the same.)
+qb::RowArray rows_of(const void* data, int64_t stride, int64_t rows) {
+    return {const_cast<void*>(data), rows > 1 ? (long long)stride : 0, 0};
+}
 
 size_t workspace_bytes_for(int32_t dtype, int64_t rows, int32_t cols) {
     if (rows == 0) return 0;
@@ -224,8 +228,8 @@ qb200_status qb200_layer_norm(int32_t dtype, int32_t param_dtype, const void* d_
     QB_TRY(check_param_dtype(op, dtype, param_dtype));
     QB_TRY(check_columns(op, dtype, rows, cols));
     qb::NormForwardArgs a;
-    a.x = rows_of(d_x, x_stride);
-    a.y = rows_of(d_y, y_stride);
+    a.x = rows_of(d_x, x_stride, rows);
+    a.y = rows_of(d_y, y_stride, rows);
     return run_forward(op, dtype, param_dtype, a, d_weight, d_bias, epsilon, d_mean, d_rstd, rows, cols, cuda_stream);
 }
 
@@ -240,10 +244,10 @@ qb200_status qb200_dropout_layer_norm(int32_t dtype, int32_t param_dtype, const 
     QB_TRY(check_columns(op, dtype, rows, cols));
     qb::NormForwardArgs a;
     QB_TRY(make_draw(op, rate, key, counter, d_counter, rows, cols, &a.draw));
-    a.x = rows_of(d_x, x_stride);
-    a.residual = rows_of(d_residual, residual_stride);
-    a.h = rows_of(d_h, h_stride);
-    a.y = rows_of(d_y, y_stride);
+    a.x = rows_of(d_x, x_stride, rows);
+    a.residual = rows_of(d_residual, residual_stride, rows);
+    a.h = rows_of(d_h, h_stride, rows);
+    a.y = rows_of(d_y, y_stride, rows);
     return run_forward(op, dtype, param_dtype, a, d_weight, d_bias, epsilon, d_mean, d_rstd, rows, cols, cuda_stream);
 }
 
@@ -265,9 +269,9 @@ qb200_status qb200_layer_norm_backward(int32_t dtype, int32_t param_dtype, const
     QB_TRY(check_param_dtype(op, dtype, param_dtype));
     QB_TRY(check_columns(op, dtype, rows, cols));
     qb::NormBackwardArgs a;
-    a.dy = rows_of(d_dy, dy_stride);
-    a.h = rows_of(d_x, x_stride);
-    a.dx = rows_of(d_dx, dx_stride);
+    a.dy = rows_of(d_dy, dy_stride, rows);
+    a.h = rows_of(d_x, x_stride, rows);
+    a.dx = rows_of(d_dx, dx_stride, rows);
     return run_backward(op, dtype, param_dtype, a, d_weight, d_mean, d_rstd, d_dweight, d_dbias, d_workspace, workspace_bytes, rows,
                         cols, cuda_stream);
 }
@@ -285,11 +289,11 @@ qb200_status qb200_dropout_layer_norm_backward(int32_t dtype, int32_t param_dtyp
     QB_TRY(check_columns(op, dtype, rows, cols));
     qb::NormBackwardArgs a;
     QB_TRY(make_draw(op, rate, key, counter, d_counter, rows, cols, &a.draw));
-    a.dy = rows_of(d_dy, dy_stride);
-    a.dh = rows_of(d_dh, dh_stride);
-    a.h = rows_of(d_h, h_stride);
-    a.dx = rows_of(d_dx, dx_stride);
-    a.dresidual = rows_of(d_dresidual, dresidual_stride);
+    a.dy = rows_of(d_dy, dy_stride, rows);
+    a.dh = rows_of(d_dh, dh_stride, rows);
+    a.h = rows_of(d_h, h_stride, rows);
+    a.dx = rows_of(d_dx, dx_stride, rows);
+    a.dresidual = rows_of(d_dresidual, dresidual_stride, rows);
     return run_backward(op, dtype, param_dtype, a, d_weight, d_mean, d_rstd, d_dweight, d_dbias, d_workspace, workspace_bytes, rows,
                         cols, cuda_stream);
 }
@@ -305,8 +309,8 @@ qb200_status qb200_dropout(int32_t dtype, const void* d_x, int64_t x_stride, int
     QB_TRY(check_present(op, {{"x", d_x, true}, {"y", d_y, true}}));
     QB_TRY(check_rows(op, "x", d_x, x_stride, rows, cols, dtype, false));
     QB_TRY(check_rows(op, "y", d_y, y_stride, rows, cols, dtype, true));
-    a.x = rows_of(d_x, x_stride);
-    a.y = rows_of(d_y, y_stride);
+    a.x = rows_of(d_x, x_stride, rows);
+    a.y = rows_of(d_y, y_stride, rows);
     a.rows = rows;
     a.cols = cols;
     DeviceOf device;

@@ -58,3 +58,37 @@ def test_rows_over_several_blocks_beside_other_work(cuda_device, dtype, rows, co
                 got, want = got.view, want.view
             assert nu.same_bits(got, want)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", list(nu.CODES))
+@pytest.mark.parametrize("cols", [1, 40, 128, 515, 4096, 9000])
+@pytest.mark.parametrize("stride", ["odd", (1 << 62) + 1, -(1 << 61) - 3, 0])
+def test_one_rows_strides_are_not_looked_at(cuda_device, dtype, cols, stride):
+    import torch
+
+    key, rate = qb.random.key(6), 0.3
+    weight, bias = nu.vector(nu.normal(1, cols), dtype), nu.vector(nu.normal(2, cols), dtype)
+
+    def all_calls(stride):
+        def row(seed=None):
+            made = nu.Rows(1, cols, dtype, values=None if seed is None else nu.normal(seed, 1, cols))
+            made.stride = stride
+            return made
+
+        x, residual, dy, dh = (row(seed) for seed in (3, 4, 5, 6))
+        out = [row() for _ in range(7)]
+        mean, rstd = statistics(dtype, 1)
+        sums = [torch.full_like(weight, float("nan")) for _ in range(4)]
+        nu.dropout(dtype, x, rate, key.value, 0, out[0])
+        nu.layer_norm(dtype, dtype, x, weight, bias, out[1], mean, rstd)
+        nu.layer_norm_backward(dtype, dtype, dy, x, weight, mean, rstd, out[2], sums[0], sums[1])
+        nu.dropout_layer_norm(dtype, dtype, x, residual, rate, key.value, 0, weight, bias, out[3], out[4], mean, rstd)
+        nu.dropout_layer_norm_backward(dtype, dtype, dy, dh, out[3], weight, mean, rstd, rate, key.value, 0, out[5], out[6], sums[2],
+                                       sums[3])
+        for rows in out:
+            rows.stride = cols  # the buffer's own, which torch can express
+            assert rows.outside_untouched()
+        return [rows.view for rows in out] + [mean, rstd] + sums
+
+    for got, want in zip(all_calls(cols + 1 + cols % 2 if stride == "odd" else stride), all_calls(cols)):
+        assert nu.same_bits(got, want)

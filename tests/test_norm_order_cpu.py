@@ -51,3 +51,11 @@ def test_a_clusters_blocks_meet_before_the_first_sum(kernel):
     before = rows[:met[0]]
     assert before.count("{") - before.count("}") == 1
     assert not re.search(r"\breturn\b", before[:before.index("auto fetch")])
+
+
+def test_one_rows_stride_forms_no_address():
+    # Groups and turns without a row still name a source in their copies of no bytes: with one row that is the row itself.
+    text = code("norm.cu")
+    assert "rows > 1 ? (long long)stride : 0" in body(text, "qb::RowArray rows_of(")
+    calls = re.findall(r"rows_of\(d_[^)]*\)", text)
+    assert calls and all(call.endswith(", rows)") for call in calls)
