@@ -425,8 +425,8 @@ qb200_status qb200_weight_gradient_static(int32_t dtype, const void* d_acts, con
  * Arrays of rows hold `rows` x `cols` elements of `dtype` (any of the four), a
  * row's elements next to each other, row r at data + r * stride elements.
  * Strides of arrays that are read are >= 0 (0 repeats one row), of arrays that
- * are written >= cols; with one row the stride is not looked at.  Pointers need
- * the alignment of one element.  Layer norm reads and writes 16 bytes or two
+ * are written >= cols; with one row, and beside a NULL array, the stride is not
+ * looked at.  Pointers need the alignment of one element.  Layer norm reads and writes 16 bytes or two
  * elements at a time where the rows of every array of a call start on boundaries
  * of that, dropout 16 bytes where the rows of x and y start at the same distance
  * from such a boundary; elsewhere they go one element at a time.  What lies between cols and the stride is neither

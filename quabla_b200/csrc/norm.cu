@@ -134,10 +134,11 @@ qb200_status finish(const char* op, cudaError_t e) {
      : (dtype) == QB200_F16 ? qb::launch<__half>(args, stream)                      \
                             : qb::launch<__nv_bfloat16>(args, stream))
 
-// One row's stride is not looked at, whatever it is: no address is formed with it.  (Groups and turns without a row name a
-// source in their copies of no bytes; it has to be aligned all the same.)
+// An absent array's stride is not looked at, and one row's neither, whatever it is: no address is formed with it and no
+// width chosen by it.  (Groups and turns without a row name a source in their copies of no bytes; it has to be aligned all
+// the same.)
 qb::RowArray rows_of(const void* data, int64_t stride, int64_t rows) {
-    return {const_cast<void*>(data), rows > 1 ? (long long)stride : 0, 0};
+    return {const_cast<void*>(data), data != nullptr && rows > 1 ? (long long)stride : 0, 0};
 }
 
 size_t workspace_bytes_for(int32_t dtype, int64_t rows, int32_t cols) {

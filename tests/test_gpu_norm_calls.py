@@ -4,6 +4,7 @@ on the device, with arrays laid out differently from each other, over far offset
 import pytest
 
 import quabla_b200 as qb
+from quabla_b200 import _lib
 
 import _norm_util as nu
 
@@ -91,4 +92,33 @@ def test_one_rows_strides_are_not_looked_at(cuda_device, dtype, cols, stride):
         return [rows.view for rows in out] + [mean, rstd] + sums
 
     for got, want in zip(all_calls(cols + 1 + cols % 2 if stride == "odd" else stride), all_calls(cols)):
+        assert nu.same_bits(got, want)
+
+
+@pytest.mark.parametrize("dtype", list(nu.CODES))
+@pytest.mark.parametrize("stride", [1, -3, (1 << 62) + 1])
+def test_strides_of_absent_arrays_are_not_looked_at(cuda_device, dtype, stride):
+    # Rows that go 16 bytes at a time go so whatever stands beside a NULL, and their sums run in the same order.
+    import torch
+
+    rows, cols, rate, key, code = 200, 1000, 0.25, 17, nu.CODES[dtype]
+    lib = _lib.load()
+    x, dy = normal_rows(1, rows, cols, dtype), normal_rows(2, rows, cols, dtype)
+    weight = nu.vector(1 + 0.2 * nu.normal(3, cols), dtype)
+
+    def both(stride):
+        y, dx = nu.Rows(rows, cols, dtype), nu.Rows(rows, cols, dtype)
+        mean, rstd = statistics(dtype, rows)
+        dweight, dbias = torch.full_like(weight, float("nan")), torch.full_like(weight, float("nan"))
+        space = nu.workspace(dtype, rows, cols)
+        _lib.check(lib.qb200_dropout_layer_norm(code, code, x.ptr, cols, None, stride, rows, cols, rate, key, 0, None,
+                                                weight.data_ptr(), None, nu.EPSILON, None, stride, y.ptr, cols, mean.data_ptr(),
+                                                rstd.data_ptr(), nu.stream()))
+        _lib.check(lib.qb200_dropout_layer_norm_backward(code, code, dy.ptr, cols, None, stride, x.ptr, cols, rows, cols,
+                                                         weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rate, key, 0, None,
+                                                         dx.ptr, cols, None, stride, dweight.data_ptr(), dbias.data_ptr(),
+                                                         space.data_ptr(), space.numel(), nu.stream()))
+        return y.view, mean, rstd, dx.view, dweight, dbias
+
+    for got, want in zip(both(stride), both(0)):
         assert nu.same_bits(got, want)
