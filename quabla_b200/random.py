@@ -59,7 +59,7 @@ def _mix_scalar(z: int) -> int:
 def _stream(key: int, count: int, first: int = 0) -> np.ndarray:
     """`count` outputs of the SplitMix64 stream seeded by `key`, from output `first` on."""
     with np.errstate(over="ignore"):
-        z = np.uint64(key) + (np.arange(1, count + 1, dtype=np.uint64) + np.uint64(first)) * np.uint64(_GAMMA)
+        z = np.uint64((key + first * _GAMMA) & _MASK) + np.arange(1, count + 1, dtype=np.uint64) * np.uint64(_GAMMA)
         z = (z ^ (z >> np.uint64(30))) * np.uint64(_M1)
         z = (z ^ (z >> np.uint64(27))) * np.uint64(_M2)
         return z ^ (z >> np.uint64(31))
