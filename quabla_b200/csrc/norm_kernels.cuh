@@ -670,10 +670,7 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
         if (RESIDUAL) dh += p.dh.advance;
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        fetch(ring.stage(s), s);
-        ring.settle(ring.stage(s), pending);
-    }
+    for (int s = 0; s < STAGES - 1; ++s) fetch(ring.stage(s), s);
 
     const DrawStream draws(p.draw);
     const A scale = (A)p.draw.scale, inverse = (A)1 / (A)p.cols;
@@ -750,7 +747,6 @@ norm_backward_kernel(const __grid_constant__ NormBackwardArgs p, const RowShape 
                 }
                 if (live) place.store(dx + r * p.dx.stride, d, whole);
             }
-            ring.settle(free, pending);
             free = now;
             now = now == ring.stage(STAGES - 1) ? ring.stage(0) : now + Ring::STAGE_BYTES;
             row += place.step;
