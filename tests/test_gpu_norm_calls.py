@@ -122,3 +122,196 @@ def test_strides_of_absent_arrays_are_not_looked_at(cuda_device, dtype, stride):
 
     for got, want in zip(both(stride), both(0)):
         assert nu.same_bits(got, want)
+
+
+# ---- sums over very many rows ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,params", nu.TYPE_PAIRS)
+@pytest.mark.parametrize("rows,cols", [(262147, 16), (262147, 17), (100003, 64), (50021, 130), (9001, 1024), (5003, 4101), (601, 9000)])
+def test_no_row_is_missing_from_the_sums(cuda_device, dtype, params, rows, cols):
+    # Small whole numbers, mean 0 and rstd 1: every partial sum is a whole number below 2^24, so the sums are exact in any
+    # order, and rounded once where the parameters have 16 bits.
+    import torch
+
+    generator = torch.Generator(device="cuda").manual_seed(rows + cols)
+
+    def whole(low, high):
+        return torch.randint(low, high + 1, (rows, cols), device="cuda", generator=generator)
+
+    # A mean of a half: with terms of mean 0 a sum could hide a row behind its own rounding in 16 bits.
+    dy, x = whole(-1, 2), whole(0, 2)
+    dweight, dbias = (dy * x).sum(0), dy.sum(0)
+    assert max((dy * x).abs().sum(0).max(), dy.abs().sum(0).max()) < 2**24
+    dy, x = nu.Rows(rows, cols, dtype, values=dy), nu.Rows(rows, cols, dtype, values=x)
+    mean, rstd = (torch.full((rows,), v, dtype=nu.statistics_type(dtype), device="cuda") for v in (0.0, 1.0))
+    for residual in (False, True):
+        dx = nu.Rows(rows, cols, dtype)
+        got = [torch.full((cols,), float("nan"), dtype=nu.torch_type(params), device="cuda") for _ in range(2)]
+        if residual:
+            nu.dropout_layer_norm_backward(dtype, params, dy, dy, x, None, mean, rstd, 0.5, 9, 0, dx, None, *got)
+        else:
+            nu.layer_norm_backward(dtype, params, dy, x, None, mean, rstd, dx, *got)
+        for sums, want in zip(got, (dweight, dbias)):
+            assert (sums == want.to(sums.dtype)).all()
+
+
+# ---- arrays that are laid out differently ------------------------------------------------------
+
+# Several turns of the kernels' rows, but for the first two of each width: rows that share a warp, whole warps, several
+# blocks.
+DIFFERENT = [(3, 40), (40000, 40), (2600, 515), (900, 1024), (3, 5120), (200, 9000)]
+
+
+@pytest.mark.parametrize("dtype", list(nu.CODES))
+@pytest.mark.parametrize("rows,cols", DIFFERENT)
+@pytest.mark.parametrize("odd", ["x", "residual", "h", "y", "all"])
+def test_forward_arrays_with_strides_and_boundaries_of_their_own(cuda_device, dtype, rows, cols, odd):
+    # One array off every boundary decides how all of them are read; strides are all different.
+    key, rate, counter = qb.random.key(31), 0.3, 2**32 - 5
+    layout = {name: dict(pad=-cols % 8 + 8 * i, shift=0) for i, name in enumerate(("x", "residual", "h", "y"))}
+    for i, name in enumerate(layout):
+        if odd in (name, "all"):
+            layout[name] = dict(pad=2 * i + 1 + cols % 2, shift=i + 1)
+    x, residual = normal_rows(1, rows, cols, dtype, **layout["x"]), normal_rows(2, rows, cols, dtype, **layout["residual"])
+    h, y = nu.Rows(rows, cols, dtype, **layout["h"]), nu.Rows(rows, cols, dtype, **layout["y"])
+    weight, bias = nu.vector(1 + 0.2 * nu.normal(3, cols), dtype), nu.vector(nu.normal(4, cols), dtype)
+    mean, rstd = statistics(dtype, rows)
+    nu.dropout_layer_norm(dtype, dtype, x, residual, rate, key.value, counter, weight, bias, h, y, mean, rstd)
+    branch = nu.dropped(x.wide(), nu.mask(key, rows, cols, rate, counter), rate)
+    want, u = residual.wide() + branch, nu.unit(dtype)
+    # Scale and product round once each, the sum once, then h's own type.
+    assert ((h.wide() - want).abs() <= nu.half_step(dtype) * (1 + 8 * u) * want.abs() + 4 * u * (branch.abs() + want.abs())
+            + nu.tiny(dtype)).all()
+    nu.check_forward(dtype, want, weight, bias, y, mean, rstd)
+    assert h.outside_untouched() and y.outside_untouched()
+    if odd in ("x", "y"):
+        y = nu.Rows(rows, cols, dtype, **layout["y"])
+        nu.layer_norm(dtype, dtype, x, weight, bias, y, mean, rstd)
+        nu.check_forward(dtype, x.wide(), weight, bias, y, mean, rstd)
+        assert y.outside_untouched()
+
+
+@pytest.mark.parametrize("dtype", list(nu.CODES))
+@pytest.mark.parametrize("rows,cols", DIFFERENT)
+@pytest.mark.parametrize("odd", ["dy", "dh", "h", "dx", "dresidual", "all"])
+def test_backward_arrays_with_strides_and_boundaries_of_their_own(cuda_device, dtype, rows, cols, odd):
+    import torch
+
+    key, rate, counter = qb.random.key(32), 0.3, 2**62 + 1
+    layout = {name: dict(pad=-cols % 8 + 8 * i, shift=0) for i, name in enumerate(("dy", "dh", "h", "dx", "dresidual"))}
+    for i, name in enumerate(layout):
+        if odd in (name, "all"):
+            layout[name] = dict(pad=2 * i + 1 + cols % 2, shift=i + 1)
+    dy, dh = normal_rows(1, rows, cols, dtype, 0.1, **layout["dy"]), normal_rows(2, rows, cols, dtype, 0.1, **layout["dh"])
+    h = normal_rows(3, rows, cols, dtype, **layout["h"])
+    dx, dresidual = nu.Rows(rows, cols, dtype, **layout["dx"]), nu.Rows(rows, cols, dtype, **layout["dresidual"])
+    weight = nu.vector(1 + 0.2 * nu.normal(4, cols), dtype)
+    wide = h.wide()
+    mean = wide.mean(1).to(nu.statistics_type(dtype))
+    rstd = (((wide - wide.mean(1, keepdim=True)) ** 2).mean(1) + nu.EPSILON).rsqrt().to(mean.dtype)
+    dweight, dbias = torch.full_like(weight, float("nan")), torch.full_like(weight, float("nan"))
+    nu.dropout_layer_norm_backward(dtype, dtype, dy, dh, h, weight, mean, rstd, rate, key.value, counter, dx, dresidual, dweight,
+                                   dbias)
+    nu.check_backward(dtype, dtype, dy, h, weight, mean, rstd, dx, dweight, dbias, dh, dresidual,
+                      nu.mask(key, rows, cols, rate, counter), rate)
+    assert dx.outside_untouched() and dresidual.outside_untouched()
+    if odd in ("dy", "h", "dx"):
+        dx = nu.Rows(rows, cols, dtype, **layout["dx"])
+        nu.layer_norm_backward(dtype, dtype, dy, h, weight, mean, rstd, dx, dweight, dbias)
+        nu.check_backward(dtype, dtype, dy, h, weight, mean, rstd, dx, dweight, dbias)
+        assert dx.outside_untouched()
+
+
+# ---- far offsets, high counters ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(nu.CODES))
+@pytest.mark.parametrize("cols", [40, 1000])
+def test_all_arrays_past_32_bits(cuda_device, dtype, cols):
+    # Every array's second row lies more than 2^32 elements (2^31 of the wider types) behind its first; the arrays stand
+    # beside each other in one buffer.
+    import torch
+
+    stride = (1 << 32) + 8 if dtype in ("float16", "bfloat16") else (1 << 31) + 8
+    buffer = torch.empty(stride + 10 * 1024, dtype=nu.torch_type(dtype), device="cuda")
+    for first in (0, stride):
+        buffer[first:first + 10 * 1024] = nu.Rows.SENTINEL
+
+    def far(place, seed=None):
+        rows = nu.Rows(0, cols, dtype)
+        rows.rows, rows.stride = 2, stride
+        rows.view = torch.as_strided(buffer, (2, cols), (stride, 1), place * 1024)
+        if seed is not None:
+            rows.view.copy_(nu.normal(seed, 2, cols))
+        return rows
+
+    key, rate, counter = qb.random.key(41), 0.2, 2**62 + 1
+    x, residual, h, y, dy, dh, dx, dresidual, dropped = (far(i, i + 1 if i in (0, 1, 4, 5) else None) for i in range(9))
+    mean, rstd = statistics(dtype, 2)
+    sums = [torch.full((cols,), float("nan"), dtype=nu.torch_type(dtype), device="cuda") for _ in range(2)]
+    kept = nu.mask(key, 2, cols, rate, counter)
+    nu.dropout_layer_norm(dtype, dtype, x, residual, rate, key.value, counter, None, None, h, y, mean, rstd)
+    nu.check_forward(dtype, residual.wide() + nu.dropped(x.wide(), kept, rate), None, None, y, mean, rstd)
+    nu.dropout_layer_norm_backward(dtype, dtype, dy, dh, h, None, mean, rstd, rate, key.value, counter, dx, dresidual, *sums)
+    nu.check_backward(dtype, dtype, dy, h, None, mean, rstd, dx, *sums, dh, dresidual, kept, rate)
+    nu.dropout(dtype, x, rate, key.value, counter, dropped)
+    scale = torch.tensor(1.0 / (1.0 - rate), dtype=nu.statistics_type(dtype), device="cuda")
+    assert (dropped.view == torch.where(kept, x.view.to(scale.dtype) * scale, 0.0).to(x.view.dtype)).all()
+    nu.layer_norm(dtype, dtype, x, None, None, y, mean, rstd)
+    nu.check_forward(dtype, x.wide(), None, None, y, mean, rstd)
+    nu.layer_norm_backward(dtype, dtype, dy, x, None, mean, rstd, dx, *sums)
+    nu.check_backward(dtype, dtype, dy, x, None, mean, rstd, dx, *sums)
+    for first in (0, stride):
+        between = buffer[first:first + 10 * 1024].view(10, 1024)
+        assert (between[:, cols:] == nu.Rows.SENTINEL).all() and (between[9] == nu.Rows.SENTINEL).all()
+
+
+@pytest.mark.parametrize("dtype", list(nu.CODES))
+@pytest.mark.parametrize("rows,cols,pad,shift", [(1, 1, 0, 0), (37, 33, 0, 1), (70, 96, 0, 0), (300, 34, 0, 0), (5, 4097, 3, 0), (3, 9000, 0, 0)])
+@pytest.mark.parametrize("counter", [1, 2**32 - 5, 2**33 + 1, 2**62 + 1, 2**64 - 2**17])
+@pytest.mark.parametrize("rate", [0.3, 0.5 + 2.0**-32])
+def test_residual_masks_at_high_counters(cuda_device, dtype, rows, cols, pad, shift, counter, rate):
+    import torch
+
+    key = qb.random.key(0xFEDCBA9876543210)
+    kept = nu.mask(key, rows, cols, rate, counter)
+    one = nu.Rows(rows, cols, dtype, pad, shift, torch.ones(rows, cols, dtype=torch.float64, device="cuda"))
+    h, y, dx, dresidual = (nu.Rows(rows, cols, dtype, pad, shift) for _ in range(4))
+    mean, rstd = statistics(dtype, rows)
+    nu.dropout_layer_norm(dtype, dtype, one, None, rate, key.value, counter, None, None, h, y, mean, rstd)
+    assert ((h.view != 0) == kept).all()
+    # With dy = 0 the gradient is dh behind the same mask.
+    zero = nu.Rows(rows, cols, dtype, pad, shift, torch.zeros(rows, cols, dtype=torch.float64, device="cuda"))
+    nu.dropout_layer_norm_backward(dtype, dtype, zero, one, h, None, mean, rstd, rate, key.value, counter, dx, dresidual, None, None)
+    assert (dresidual.view == 1).all() and ((dx.view != 0) == kept).all()
+    assert nu.same_bits(dx.view, h.view)
+
+
+@pytest.mark.parametrize("dtype", list(nu.CODES))
+@pytest.mark.parametrize("rows,cols", [(40, 64), (40, 65), (41, 1024), (5, 9000)])
+def test_nans_stay_in_their_rows_and_columns(cuda_device, dtype, rows, cols):
+    # Two 16-bit rows share a turn: what one holds must not reach the other, nor the columns of the sums that it is not in.
+    import torch
+
+    x, dy, dh = (normal_rows(seed, rows, cols, dtype) for seed in (1, 2, 3))
+    mean, rstd = statistics(dtype, rows)
+    y = nu.Rows(rows, cols, dtype)
+    nu.layer_norm(dtype, dtype, x, None, None, y, mean, rstd)
+
+    def backward():
+        dx = nu.Rows(rows, cols, dtype)
+        sums = [torch.full((cols,), 5.0, dtype=nu.torch_type(dtype), device="cuda") for _ in range(2)]
+        nu.dropout_layer_norm_backward(dtype, dtype, dy, dh, x, None, mean, rstd, 0.0, 0, 0, dx, None, *sums)
+        return dx.view, *sums
+
+    clean_y, clean = y.view.clone(), backward()
+    dy.view[2, cols // 3] = float("nan")
+    dx, dweight, dbias = backward()
+    row, column = torch.arange(rows, device="cuda") == 2, torch.arange(cols, device="cuda") == cols // 3
+    assert torch.isnan(dx[2]).all() and nu.same_bits(dx[~row], clean[0][~row])
+    for got, want in ((dweight, clean[1]), (dbias, clean[2])):
+        assert torch.isnan(got[column]).all() and nu.same_bits(got[~column], want[~column])
+    x.view[2, cols - 1] = float("nan")
+    nu.layer_norm(dtype, dtype, x, None, None, y, mean, rstd)
+    assert torch.isnan(y.view[2]).all() and nu.same_bits(y.view[~row], clean_y[~row])
