@@ -426,11 +426,12 @@ qb200_status qb200_weight_gradient_static(int32_t dtype, const void* d_acts, con
  * row's elements next to each other, row r at data + r * stride elements.
  * Strides of arrays that are read are >= 0 (0 repeats one row), of arrays that
  * are written >= cols; with one row, and beside a NULL array, the stride is not
- * looked at.  Pointers need the alignment of one element.  Layer norm reads and writes 16 bytes or two
- * elements at a time where the rows of every array of a call start on boundaries
- * of that, dropout 16 bytes where the rows of x and y start at the same distance
- * from such a boundary; elsewhere they go one element at a time.  What lies between cols and the stride is neither
- * read nor written.  Zero rows are valid (the sums over rows are then zero).  Parameters
+ * looked at.  Pointers need the alignment of one element.  Layer norm reads and
+ * writes 16 bytes or two elements at a time where the rows of every array of a
+ * call start on boundaries of that, dropout 16 bytes where the rows of x and y
+ * start at the same distance from such a boundary; elsewhere they go one element
+ * at a time.  What lies between cols and the stride is neither read nor written.
+ * Zero rows are valid (the sums over rows are then zero).  Parameters
  * (weight, bias and their gradients) are of `param_dtype`: the rows' dtype, or
  * QB200_F32 beside 16-bit rows; either may be NULL and then stands for 1 or 0.
  * Statistics (mean, rstd) and all sums are float32, float64 for float64 rows;
@@ -468,7 +469,7 @@ qb200_status qb200_layer_norm(int32_t dtype, int32_t param_dtype, const void* d_
                               int32_t cols, const void* d_weight, const void* d_bias, double epsilon, void* d_y,
                               int64_t y_stride, void* d_mean, void* d_rstd, void* cuda_stream);
 
-/* Bytes of workspace of a backward pass over `rows` x `cols` (at most 19 MiB): partial sums of
+/* Bytes of workspace of a backward pass over `rows` x `cols` (at most 9.25 MiB): partial sums of
  * the parameters' gradients, one row for each group of thread blocks. */
 qb200_status qb200_layer_norm_workspace(int32_t dtype, int64_t rows, int32_t cols, size_t* nbytes);
 
