@@ -43,7 +43,7 @@ struct DrawStream {
     __device__ __forceinline__ bool low_kept(unsigned long long z) const { return (unsigned int)(z ^ (z >> 31)) >= threshold; }
     // The last step changes no more of the high half than its lowest bit, and that only where its highest is set.  A
     // threshold up to 2^31 cannot tell, nor can an even one; for an odd one above, FLIP (the integer units are what
-    // bounds 16-bit dropout: without it two of their eleven instructions for an element's half of a word go).
+    // bounds 16-bit dropout: without the last step the high half takes two of their instructions less).
     template <bool FLIP> __device__ __forceinline__ bool high_kept(unsigned long long z) const {
         return ((unsigned int)(z >> 32) ^ (FLIP ? 1u : 0u)) >= threshold;
     }

@@ -10,7 +10,7 @@
 // registers, not over memory).  Sums, statistics and gradients are float32 (float64 for float64 rows); the rows' type is
 // rounded to once, on the way out.  Sums run in a fixed order: results repeat bit for bit.
 //
-// All of it is bound by memory in principle (4 to 10 bytes of traffic for a 16-bit element against 10 to 30 instructions);
+// All of it is bound by memory in principle (4 to 10 bytes of traffic for a 16-bit element against 12 to 36 instructions);
 // what kept the first versions from it was instruction issue and the latency of the rows' sums, so the layout below is about
 // few instructions for an element and rows that are fetched ahead.  Rates are given as a share of the measured copy rate of
 // 6542 GB/s, times are of one B200 with inputs that change from call to call.
@@ -470,7 +470,7 @@ __device__ __forceinline__ void by_draws(const DrawStream& draws, int cols, F&& 
 
 // RESIDUAL: x passes through dropout and may be added to a residual; otherwise h = x.
 // 8192 x 4096 bfloat16: 26.7 us, 77 % (32768 rows: 88 us, 92 %: launch and first rows are 4 us); float32 45 us, 91 %.  The
-// residual form of 4096 x 4096 bfloat16 32 us, 64 %, 28.5 without dropout: the draws are 9 integer instructions an element
+// residual form of 4096 x 4096 bfloat16 32 us, 64 %, 28.5 without dropout: the draws are 10 integer instructions an element
 // and 16 warps an SM do not hide all of them.  More warps with fewer registers, parameters in shared memory, and draws for
 // the next turn during this one's sums all measured slower or the same.
 template <typename T, int V, int SPAN, bool RESIDUAL>
@@ -865,7 +865,7 @@ __device__ __forceinline__ void drop_packs(const DrawStream& draws, long long in
 // long row (what a contiguous array is) and many rows are two kernels: in the one row the four packs that a thread has on
 // their way are a constant distance apart in the stream of words; of many rows a thread has two (8192 x 4095 bfloat16 55 us, with
 // four 62).
-// 16384 x 8192 bfloat16: 108 us, 76 %: the integer units are 71 % busy (11 of 17.5 instructions for an element, 4 bytes of
+// 16384 x 8192 bfloat16: 108 us, 76 %: the integer units are 71 % busy (10 of 17.5 instructions for an element, 4 bytes of
 // traffic); 8192 x 8192 float32 86 us, 95 %.
 __host__ __device__ constexpr int dropout_depth(bool one_row) { return one_row ? 4 : 2; }
 template <typename T, int V, bool ONE_ROW>
