@@ -315,3 +315,45 @@ def test_nans_stay_in_their_rows_and_columns(cuda_device, dtype, rows, cols):
     x.view[2, cols - 1] = float("nan")
     nu.layer_norm(dtype, dtype, x, None, None, y, mean, rstd)
     assert torch.isnan(y.view[2]).all() and nu.same_bits(y.view[~row], clean_y[~row])
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_in_order_may_share_a_workspace(cuda_device, captured):
+    # The sums of one call are joined by a kernel that starts while its rows are still in work; the next call's rows must
+    # not reach the workspace before it has read them.
+    import torch
+
+    sizes = [("bfloat16", 3000, 1024), ("float32", 5000, 65), ("float32", 40000, 16), ("float64", 300, 4100), ("bfloat16", 37, 20000)]
+    space = torch.full((9_699_328,), 255, dtype=torch.uint8, device="cuda")
+    made = []
+    for i, (dtype, rows, cols) in enumerate(sizes):
+        x, dy = normal_rows(2 * i, rows, cols, dtype), normal_rows(2 * i + 1, rows, cols, dtype, 0.1)
+        y = nu.Rows(rows, cols, dtype)
+        mean, rstd = statistics(dtype, rows)
+        nu.layer_norm(dtype, dtype, x, None, None, y, mean, rstd)
+        sums = [torch.full((cols,), float("nan"), dtype=nu.torch_type(dtype), device="cuda") for _ in range(2)]
+        made.append((dtype, dy, x, mean, rstd, nu.Rows(rows, cols, dtype), sums))
+
+    def calls():
+        for dtype, dy, x, mean, rstd, dx, sums in made:
+            nu.layer_norm_backward(dtype, dtype, dy, x, None, mean, rstd, dx, *sums, space=space)
+
+    calls()
+    torch.cuda.synchronize()
+    want = []
+    for dtype, dy, x, mean, rstd, dx, sums in made:
+        nu.check_backward(dtype, dtype, dy, x, None, mean, rstd, dx, *sums)
+        want.append([t.clone() for t in sums])
+    run = calls
+    if captured:
+        on, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=on):
+            calls()
+        run = graph.replay
+    for _ in range(20):
+        for *_, sums in made:
+            for t in sums:
+                t.fill_(float("nan"))
+        run()
+        for (*_, sums), kept in zip(made, want):
+            assert all(nu.same_bits(a, b) for a, b in zip(sums, kept))
